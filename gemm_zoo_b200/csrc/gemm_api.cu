@@ -1584,3 +1584,4 @@ extern "C" GZ_API gz_status gz_static_last_device_status(int32_t device, void* s
 
 // ------------------------------------------------------------------ K-sharded GEMM (multi-GPU)
 #include "ksharded.cuh"
+#include "microscale.cuh"

@@ -1,0 +1,493 @@
+// Host layer of the microscaled 4-bit operators (include/gemmzoo/microscale.h): argument checks, tile
+// choice, tensor maps and launches.  Included at the end of gemm_api.cu, whose helpers it uses.
+#ifndef GZ_MICROSCALE_CUH
+#define GZ_MICROSCALE_CUH
+
+#include "gemmzoo/microscale.h"
+#include "mx_gemm.cuh"
+#include "mx_quant.cuh"
+#include "mx_table.h"
+
+namespace {
+
+bool is_mx(int f) { return f == GZ_MX_FP4 || f == GZ_MX_NVFP4; }
+int mx_block(int format) { return format == GZ_MX_NVFP4 ? 16 : 32; }
+int64_t mx_groups(int format, int64_t k) { return cdiv(cdiv(k, mx_block(format)), 4); }
+bool mx_float_type(int t) { return t == GZ_DT_F16 || t == GZ_DT_BF16 || t == GZ_DT_F32; }
+bool mx_aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+constexpr int64_t kMxExtent = (int64_t(1) << 31) - 1024;  // 32-bit tile and TMA coordinates
+
+// rows x pitch addressable, without overflow
+bool mx_span_ok(int64_t rows, int64_t pitch) {
+  int64_t s;
+  return !__builtin_mul_overflow(rows, pitch, &s) && s <= (int64_t(1) << 60);
+}
+
+gz_status mx_device_ok(int device) {
+  int ndev = 0;
+  if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0) {
+    (void)cudaGetLastError();
+    return GZ_ERR_NO_DEVICE;
+  }
+  return device < ndev ? GZ_OK : GZ_ERR_INVALID_ARG;
+}
+
+// What quantisation and its inverse check alike.
+gz_status mx_quant_params(gz::mx::QuantParams* p, const void* values, int type, int layout, int64_t ld, int64_t rows,
+                          int64_t k, int format, float multiplier, const void* codes, int64_t pitch, const void* scales,
+                          int device) {
+  if (!values || !codes || !scales || rows <= 0 || k <= 0 || device < 0 || ld < 0 || pitch < 0) return GZ_ERR_INVALID_ARG;
+  if (layout != GZ_ROW_MAJOR && layout != GZ_COL_MAJOR) return GZ_ERR_INVALID_ARG;
+  if (!is_mx(format) || dtype_size(type) == 0 || !(std::fabs(multiplier) <= 3.4028234e38f) || multiplier == 0.0f)
+    return GZ_ERR_INVALID_ARG;
+  if (!mx_float_type(type)) return GZ_ERR_UNSUPPORTED;
+  if (rows > kMxExtent || k > kMxExtent) return GZ_ERR_TOO_LARGE;
+  const bool cols = layout == GZ_COL_MAJOR;
+  if (ld == 0) ld = cols ? rows : k;
+  if (pitch == 0) pitch = gz_mx_code_pitch(k);
+  if (ld < (cols ? rows : k) || pitch < gz_mx_code_pitch(k) || pitch % 16 != 0) return GZ_ERR_INVALID_ARG;
+  const int size = dtype_size(type);
+  if (!mx_span_ok(cols ? k : rows, ld) || !mx_span_ok(rows, pitch)) return GZ_ERR_TOO_LARGE;
+  if (!mx_aligned(values, size) || !mx_aligned(codes, 16) || !mx_aligned(scales, 16)) return GZ_ERR_MISALIGNED;
+  std::memset(p, 0, sizeof(*p));
+  p->rows = rows;
+  p->k = k;
+  p->ld = ld;
+  p->pitch = pitch;
+  p->code_bytes = gz_mx_code_pitch(k);
+  p->groups = mx_groups(format, k);
+  p->multiplier = multiplier;
+  const uintptr_t vec = cols ? 16 : 32;  // bytes per access of the two kernels
+  p->vec = (mx_aligned(values, vec) && (ld * size) % (int64_t)vec == 0) ? 1u : 0u;
+  return GZ_OK;
+}
+
+struct MxShape {
+  int config, bn;
+  bool pair;
+};
+const MxShape kMxShapes[] = {{GZ_MX_CFG_PAIR, 256, true},
+                             {GZ_MX_CFG_SWAP_M16, 16, false},
+                             {GZ_MX_CFG_SWAP_M32, 32, false},
+                             {GZ_MX_CFG_SWAP_M64, 64, false},
+                             {GZ_MX_CFG_SWAP_M128, 128, false}};
+const MxShape* mx_shape_of(int config) {
+  for (const auto& s : kMxShapes)
+    if (s.config == config) return &s;
+  return nullptr;
+}
+
+struct MxProblem {
+  gz_mx_desc d;
+  int out_size;  // 0: quantised
+};
+
+gz_status mx_normalise(const gz_mx_desc* desc, MxProblem* pr) {
+  if (!desc || desc->struct_size != sizeof(gz_mx_desc)) return GZ_ERR_INVALID_ARG;
+  gz_mx_desc d = *desc;
+  if (d.m <= 0 || d.n <= 0 || d.k <= 0 || d.device < 0 || !is_mx(d.format)) return GZ_ERR_INVALID_ARG;
+  if (d.gated != 0 && d.gated != 1) return GZ_ERR_INVALID_ARG;
+  if (dtype_size(d.out_type) == 0 && !is_mx(d.out_type)) return GZ_ERR_INVALID_ARG;
+  if (d.flags & ~GZ_FLAG_TEST_WITHHOLD_ACC_READY) return GZ_ERR_INVALID_ARG;
+  if (d.config != GZ_MX_CFG_AUTO && !mx_shape_of(d.config)) return GZ_ERR_INVALID_ARG;
+  if (d.split != 0 && d.split != 1 && d.split != 2 && d.split != 4 && d.split != 8) return GZ_ERR_INVALID_ARG;
+  if (!mx_float_type(d.out_type) && !(is_mx(d.out_type) && d.gated)) return GZ_ERR_UNSUPPORTED;
+  if (d.m > kMxExtent || d.n > kMxExtent || d.k > kMxExtent) return GZ_ERR_TOO_LARGE;
+  const bool quantised = is_mx(d.out_type);
+  const int64_t in_pitch = gz_mx_code_pitch(d.k), out_ld = quantised ? gz_mx_code_pitch(d.n) : d.n;
+  if (d.pitch_a < 0 || d.pitch_b < 0 || d.ldc < 0 || d.ldd < 0) return GZ_ERR_INVALID_ARG;
+  if (d.pitch_a == 0) d.pitch_a = in_pitch;
+  if (d.pitch_b == 0) d.pitch_b = in_pitch;
+  if (d.ldc == 0) d.ldc = d.n;
+  if (d.ldd == 0) d.ldd = out_ld;
+  if (d.pitch_a < in_pitch || d.pitch_b < in_pitch || d.ldc < d.n || d.ldd < out_ld) return GZ_ERR_INVALID_ARG;
+  if (d.pitch_a % 16 != 0 || d.pitch_b % 16 != 0 || (quantised && d.ldd % 16 != 0)) return GZ_ERR_MISALIGNED;
+  const int64_t stride_lim = int64_t(1) << 39;  // of a tensor map
+  if (!mx_span_ok(d.m, d.pitch_a) || !mx_span_ok(d.n, d.pitch_b) || !mx_span_ok(d.m, d.ldc) || !mx_span_ok(d.m, d.ldd) ||
+      d.pitch_a > stride_lim || d.pitch_b > stride_lim)
+    return GZ_ERR_TOO_LARGE;
+  if (cdiv(d.m, 128) * cdiv(d.n, 128) > (int64_t(1) << 31) - 1) return GZ_ERR_TOO_LARGE;
+  if (d.wait_limit_ns == 0) d.wait_limit_ns = 2000000000ull;
+  pr->d = d;
+  pr->out_size = dtype_size(d.out_type);
+  return GZ_OK;
+}
+
+bool mx_shape_fits(const MxProblem& pr, const MxShape& s) { return s.pair || s.bn == 128 || pr.d.m <= s.bn; }
+
+int64_t mx_tiles(const MxProblem& pr, const MxShape& s) {
+  if (s.pair) return cdiv(pr.d.m, 256) * cdiv(pr.d.n, pr.d.gated ? 128 : 256);
+  return cdiv(pr.d.n, 128) * cdiv(pr.d.m, s.bn);
+}
+
+// CTAs that share a tile's K range: as many as keep every tile in one wave, with at least two K blocks
+// each (a CTA's set-up and the meeting of the partial sums cost about as much as two).
+int mx_split(const MxProblem& pr, const MxShape& s, int sm_count) {
+  if (s.pair) return 1;
+  const int64_t tiles = mx_tiles(pr, s), k_blocks = cdiv(pr.d.k, 256);
+  // clusters of eight leave SMs over in each GPC: 16 of them fit
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sm_count - (split == 4 ? 20 : split == 2 ? 16 : 0) && k_blocks >= 4 * split) split *= 2;
+  return split;
+}
+
+int mx_choose(const MxProblem& pr, int sm_count) {
+  double best = 0;
+  int best_cfg = GZ_MX_CFG_SWAP_M128;
+  const double k_blocks = double(cdiv(pr.d.k, 256));
+  for (const auto& s : kMxShapes) {
+    if (!mx_shape_fits(pr, s)) continue;
+    const int64_t units = s.pair ? sm_count / 2 : sm_count;
+    if (units <= 0) continue;
+    const int64_t tiles = mx_tiles(pr, s);
+    const int split = pr.d.split ? pr.d.split : mx_split(pr, s, sm_count);
+    const double mb = s.pair ? 1.0 : pr.d.gated ? 2.0 : 1.0;
+    const double rows = s.pair ? 128.0 : double(s.bn);  // of the narrow side that a CTA loads
+    const double mma = s.pair ? 512.0 : 4.0 * mb * (s.bn / 2.0 > 32.0 + s.bn / 4.0 ? s.bn / 2.0 : 32.0 + s.bn / 4.0);
+    const double bytes = (128.0 * mb + rows) * 128.0 + 512.0 * (pr.d.format == GZ_MX_NVFP4 ? 4 : 2) * (mb + (s.pair ? 2 : 1));
+    double per_block = mma > bytes / 48.0 ? mma : bytes / 48.0;
+    if (per_block < 250.0) per_block = 250.0;
+    const double waves = double(cdiv(tiles * split, units));
+    const double fixed = (s.pair ? 6000.0 : 3000.0) + 8.0 * s.bn * mb;
+    const double cost = waves * (k_blocks / split * per_block + 500.0) + fixed + (split > 1 ? 1500.0 : 0.0);
+    if (best == 0 || cost < best) {
+      best = cost;
+      best_cfg = s.config;
+    }
+  }
+  return best_cfg;
+}
+
+gz::MxEntry mx_entry_of(const MxProblem& pr, int config) {
+  return pr.d.format == GZ_MX_NVFP4 ? gz::mx_kernels_nvfp4(config, pr.d.gated != 0)
+                                    : gz::mx_kernels_fp4(config, pr.d.gated != 0);
+}
+
+gz_status mx_resolve(const MxProblem& pr, int sm_count, gz_mx_plan_info* info) {
+  const int config = pr.d.config == GZ_MX_CFG_AUTO ? mx_choose(pr, sm_count) : pr.d.config;
+  const MxShape& s = *mx_shape_of(config);
+  if (!mx_shape_fits(pr, s)) return GZ_ERR_UNSUPPORTED;
+  const int64_t tiles = mx_tiles(pr, s);
+  int split = pr.d.split ? pr.d.split : mx_split(pr, s, sm_count);
+  if (s.pair && split != 1) return GZ_ERR_UNSUPPORTED;
+  // a shared K range is one wave of clusters, each CTA with a part of it
+  if (split > 1 && (tiles * split > sm_count || cdiv(pr.d.k, 256) < split)) return GZ_ERR_UNSUPPORTED;
+  const gz::MxEntry e = mx_entry_of(pr, config);
+  std::memset(info, 0, sizeof(*info));
+  info->config = config;
+  info->split = split;
+  info->tile_m = s.pair ? 256 : s.bn;
+  info->tile_n = s.pair ? (pr.d.gated ? 128 : 256) : 128;
+  info->tile_k = 256;
+  info->stages = e.stages;
+  info->smem_bytes = e.smem_bytes;
+  const int64_t units = s.pair ? sm_count / 2 : split > 1 ? tiles : sm_count;
+  if (units <= 0) return GZ_ERR_UNSUPPORTED;
+  info->grid = (int32_t)((tiles < units ? tiles : units) * (s.pair ? 2 : split));
+  info->out_tma = (s.pair && pr.out_size != 0 && (pr.d.ldd * pr.out_size) % 16 == 0 &&
+                   pr.d.ldd * pr.out_size < (int64_t(1) << 40)) ? 1 : 0;
+  info->tiles = tiles;
+  return GZ_OK;
+}
+
+bool mx_encode(CUtensorMap* tm, CUtensorMapDataType type, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
+               uint64_t stride1, uint64_t stride2, uint32_t b0, uint32_t b1, CUtensorMapSwizzle swizzle, bool promote) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) {
+    g_last_cuda_error = "cuTensorMapEncodeTiled entry point not available";
+    return false;
+  }
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {stride1, stride2};
+  cuuint32_t box[3] = {b0, b1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(tm, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swizzle, promote ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    char buf[96];
+    std::snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    g_last_cuda_error = buf;
+    return false;
+  }
+  return true;
+}
+
+}  // namespace
+
+struct gz_mx_plan {
+  MxProblem pr;
+  gz_mx_plan_info info;
+  gz::MxEntry entry;
+  gz::MxParams base;  // everything that does not depend on the operands of a call
+  uint32_t* status_dev;
+};
+
+namespace {
+
+// Tensor maps of one operand: codes in boxes of `box_rows` rows x 128 bytes, scales in boxes of one row
+// group x one stage's tiles.  Bytes behind ceil(k / 2) and tiles behind the last are read as zero.
+bool mx_encode_operand(const gz_mx_plan* pl, CUtensorMap* codes_map, CUtensorMap* scales_map, const void* codes,
+                       const void* scales, int64_t rows, int64_t pitch, uint32_t box_rows) {
+  const gz_mx_desc& d = pl->pr.d;
+  const uint64_t groups = (uint64_t)mx_groups(d.format, d.k);
+  return mx_encode(codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, (uint64_t)cdiv(d.k, 2), (uint64_t)rows, 1, (uint64_t)pitch,
+                   (uint64_t)pitch * (uint64_t)rows, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B, true) &&
+         mx_encode(scales_map, CU_TENSOR_MAP_DATA_TYPE_INT32, scales, 128, groups, (uint64_t)cdiv(rows, 128), 512,
+                   512 * groups, 128, d.format == GZ_MX_NVFP4 ? 4 : 2, CU_TENSOR_MAP_SWIZZLE_NONE, true);
+}
+
+// a x b (and, gated, a x up) into p->d; the caller has filled the epilogue's part of *p.
+gz_status mx_launch(gz_mx_plan* pl, gz::MxParams* p, const void* a, const void* a_scales, const void* b,
+                    const void* b_scales, const void* up, const void* up_scales, cudaStream_t stream) {
+  const gz_mx_desc& d = pl->pr.d;
+  const MxShape& s = *mx_shape_of(pl->info.config);
+  gz::MxMaps maps;
+  bool ok;
+  if (s.pair)
+    ok = mx_encode_operand(pl, &maps.wide, &maps.wide_scales, a, a_scales, d.m, d.pitch_a, 128) &&
+         mx_encode_operand(pl, &maps.narrow, &maps.narrow_scales, b, b_scales, d.n, d.pitch_b, 128);
+  else
+    ok = mx_encode_operand(pl, &maps.wide, &maps.wide_scales, b, b_scales, d.n, d.pitch_b, 128) &&
+         mx_encode_operand(pl, &maps.narrow, &maps.narrow_scales, a, a_scales, d.m, d.pitch_a, (uint32_t)s.bn);
+  if (ok && up) ok = mx_encode_operand(pl, &maps.up, &maps.up_scales, up, up_scales, d.n, d.pitch_b, 128);
+  if (!ok) return GZ_ERR_CUDA;
+  if (!up) {  // unused by the kernel
+    maps.up = maps.narrow;
+    maps.up_scales = maps.narrow_scales;
+  }
+  p->out_tma = (pl->info.out_tma && mx_aligned(p->d, 16)) ? 1u : 0u;
+  if (p->out_tma) {
+    const bool f32 = d.out_type == GZ_DT_F32;
+    if (!mx_encode(&maps.d, tmap_type(d.out_type), p->d, (uint64_t)d.n, (uint64_t)d.m, 1, (uint64_t)(d.ldd * pl->pr.out_size),
+                   (uint64_t)(d.ldd * pl->pr.out_size) * (uint64_t)d.m, 32, 32,
+                   f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, false))
+      return GZ_ERR_CUDA;
+  } else {
+    maps.d = maps.wide;  // unused by the kernel
+  }
+  if (!cuda_ok(pl->entry.launch(maps, *p, pl->info.grid, s.pair ? 2 : pl->info.split, stream), "kernel launch"))
+    return GZ_ERR_CUDA;
+  return GZ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+GZ_API int64_t gz_mx_code_pitch(int64_t k) { return k <= 0 || k > kMxExtent ? -1 : cdiv(k, 32) * 16; }
+
+GZ_API int64_t gz_mx_scale_bytes(int32_t format, int64_t rows, int64_t k) {
+  if (!is_mx(format) || rows <= 0 || k <= 0 || rows > kMxExtent || k > kMxExtent) return -1;
+  return cdiv(rows, 128) * mx_groups(format, k) * 512;
+}
+
+GZ_API gz_status gz_mx_quantize(const void* src, int32_t src_type, int32_t layout, int64_t ld, int64_t rows, int64_t k,
+                                int32_t format, float multiplier, void* codes, int64_t pitch, void* scales,
+                                int32_t device, void* stream) {
+  gz::mx::QuantParams p;
+  gz_status st = mx_quant_params(&p, src, src_type, layout, ld, rows, k, format, multiplier, codes, pitch, scales, device);
+  if (st != GZ_OK) return st;
+  const bool nv = format == GZ_MX_NVFP4, cols = layout == GZ_COL_MAJOR;
+  int64_t blocks;
+  if (cols) {
+    blocks = cdiv(rows, 128) * 2 * cdiv(k, 128);
+  } else {
+    const int64_t word = nv ? 4 : 8;  // 16-element chunks per word of scales
+    const int64_t per_row = cdiv(cdiv(k, 16), word) * word;
+    p.per_row = (uint32_t)per_row;
+    p.items = cdiv(rows, 128) * 128 * per_row;
+    blocks = cdiv(p.items, 256);
+  }
+  if (blocks > kMxExtent) return GZ_ERR_TOO_LARGE;
+  if ((st = mx_device_ok(device)) != GZ_OK) return st;
+  DeviceGuard guard(device);
+  if (!guard.ok()) return GZ_ERR_CUDA;
+  p.in = src;
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = static_cast<uint8_t*>(scales);
+  if (!cuda_ok(gz::mx_launch_quantize(src_type, nv, cols, p, blocks, static_cast<cudaStream_t>(stream)), "kernel launch"))
+    return GZ_ERR_CUDA;
+  return GZ_OK;
+}
+
+GZ_API gz_status gz_mx_dequantize(const void* codes, int64_t pitch, const void* scales, int32_t format, int64_t rows,
+                                  int64_t k, float multiplier, void* dst, int32_t dst_type, int32_t layout, int64_t ld,
+                                  int32_t device, void* stream) {
+  gz::mx::QuantParams p;
+  gz_status st = mx_quant_params(&p, dst, dst_type, layout, ld, rows, k, format, multiplier, codes, pitch, scales, device);
+  if (st != GZ_OK) return st;
+  const bool nv = format == GZ_MX_NVFP4, cols = layout == GZ_COL_MAJOR;
+  int64_t blocks;
+  if (cols) {
+    blocks = cdiv(rows, gz::mx::COL_ROWS) * cdiv(k, gz::mx::COL_K);
+  } else {
+    p.per_row = (uint32_t)cdiv(k, 16);
+    p.items = rows * (int64_t)p.per_row;
+    blocks = cdiv(p.items, 256);
+  }
+  if (blocks > kMxExtent) return GZ_ERR_TOO_LARGE;
+  if ((st = mx_device_ok(device)) != GZ_OK) return st;
+  DeviceGuard guard(device);
+  if (!guard.ok()) return GZ_ERR_CUDA;
+  p.out = dst;
+  p.codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
+  p.scales = const_cast<uint8_t*>(static_cast<const uint8_t*>(scales));
+  if (!cuda_ok(gz::mx_launch_dequantize(dst_type, nv, cols, p, blocks, static_cast<cudaStream_t>(stream)), "kernel launch"))
+    return GZ_ERR_CUDA;
+  return GZ_OK;
+}
+
+GZ_API gz_status gz_mx_desc_validate(const gz_mx_desc* desc, int sm_count, gz_mx_plan_info* info) {
+  MxProblem pr;
+  gz_status st = mx_normalise(desc, &pr);
+  if (st != GZ_OK) return st;
+  gz_mx_plan_info tmp;
+  st = mx_resolve(pr, sm_count > 0 ? sm_count : 148, &tmp);
+  if (st == GZ_OK && info) *info = tmp;
+  return st;
+}
+
+GZ_API gz_status gz_mx_plan_create(gz_mx_plan** out, const gz_mx_desc* desc) {
+  if (!out) return GZ_ERR_INVALID_ARG;
+  *out = nullptr;
+  MxProblem pr;
+  gz_status st = mx_normalise(desc, &pr);
+  if (st != GZ_OK) return st;
+  if ((st = mx_device_ok(pr.d.device)) != GZ_OK) return st;
+  int major = 0, sms = 0;
+  if (!cuda_ok(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, pr.d.device), "device attribute") ||
+      !cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, pr.d.device), "device attribute"))
+    return GZ_ERR_CUDA;
+  if (major != 10) return GZ_ERR_NO_DEVICE;
+  gz_mx_plan_info info;
+  if ((st = mx_resolve(pr, sms, &info)) != GZ_OK) return st;
+  DeviceGuard guard(pr.d.device);
+  if (!guard.ok()) return GZ_ERR_CUDA;
+  gz_mx_plan* pl = new (std::nothrow) gz_mx_plan();
+  if (!pl) return GZ_ERR_OUT_OF_MEMORY;
+  pl->pr = pr;
+  pl->info = info;
+  pl->entry = mx_entry_of(pr, info.config);
+  pl->status_dev = nullptr;
+  if (!cuda_ok(pl->entry.attr(), "cudaFuncSetAttribute(max dynamic shared memory)") ||
+      !cuda_ok(cudaMalloc(&pl->status_dev, 4 * sizeof(uint32_t)), "cudaMalloc(status)") ||
+      !cuda_ok(cudaMemset(pl->status_dev, 0, 4 * sizeof(uint32_t)), "cudaMemset(status)")) {
+    if (pl->status_dev) cudaFree(pl->status_dev);
+    delete pl;
+    return GZ_ERR_CUDA;
+  }
+  const gz_mx_desc& d = pl->pr.d;
+  const MxShape& s = *mx_shape_of(info.config);
+  gz::MxParams& p = pl->base;
+  std::memset(&p, 0, sizeof(p));
+  p.grid.tiles_m = (uint32_t)(s.pair ? cdiv(d.m, 256) : cdiv(d.n, 128));
+  p.grid.tiles_n = (uint32_t)(s.pair ? cdiv(d.n, info.tile_n) : cdiv(d.m, s.bn));
+  p.grid.group_m = s.pair ? 8u : 16u;  // about 2048 rows of output per group, as for the 8- and 16-bit tiles
+  p.grid.num_tiles = p.grid.tiles_m * p.grid.tiles_n;
+  p.m = (uint32_t)d.m;
+  p.n = (uint32_t)d.n;
+  p.k_blocks = (uint32_t)cdiv(d.k, 256);
+  p.split = (uint32_t)info.split;
+  // e2m1 operands, N, scale type, M
+  p.idesc = (1u << 7) | (1u << 10) | ((uint32_t)(s.bn >> 3) << 17) | ((d.format == GZ_MX_FP4 ? 1u : 0u) << 23) |
+            ((s.pair ? 256u >> 4 : 128u >> 4) << 24);
+  p.out_type = (uint32_t)d.out_type;
+  p.test_flags = (d.flags & GZ_FLAG_TEST_WITHHOLD_ACC_READY) ? 1u : 0u;
+  p.ldc = d.ldc;
+  p.ldd = d.ldd;
+  p.d_groups = is_mx(d.out_type) ? mx_groups(d.out_type, d.n) : 0;
+  p.status = pl->status_dev;
+  p.wait_limit_ns = d.wait_limit_ns;
+  *out = pl;
+  return GZ_OK;
+}
+
+GZ_API gz_status gz_mx_plan_destroy(gz_mx_plan* pl) {
+  if (!pl) return GZ_ERR_INVALID_ARG;
+  DeviceGuard guard(pl->pr.d.device);
+  if (pl->status_dev) cudaFree(pl->status_dev);
+  delete pl;
+  return GZ_OK;
+}
+
+GZ_API gz_status gz_mx_plan_info_get(const gz_mx_plan* pl, gz_mx_plan_info* info) {
+  if (!pl || !info) return GZ_ERR_INVALID_ARG;
+  *info = pl->info;
+  return GZ_OK;
+}
+
+GZ_API gz_status gz_mx_gemm_run(gz_mx_plan* pl, const void* a, const void* a_scales, const void* b,
+                                const void* b_scales, const void* c, void* d, const float* alpha, const float* beta,
+                                const gz_epilogue* ep, void* stream) {
+  if (!pl || !a || !a_scales || !b || !b_scales || !d || !alpha || !beta || pl->pr.d.gated) return GZ_ERR_INVALID_ARG;
+  if (*beta != 0.0f && !c) return GZ_ERR_INVALID_ARG;
+  const gz_mx_desc& ds = pl->pr.d;
+  const int size = pl->pr.out_size;
+  if (!mx_aligned(a, 16) || !mx_aligned(a_scales, 16) || !mx_aligned(b, 16) || !mx_aligned(b_scales, 16) ||
+      !mx_aligned(d, size) || !mx_aligned(c, size))
+    return GZ_ERR_MISALIGNED;
+  gz::MxParams p = pl->base;
+  if (ep) {
+    if (ep->struct_size != sizeof(gz_epilogue) || ep->activation < GZ_ACT_NONE || ep->activation > GZ_ACT_SILU)
+      return GZ_ERR_INVALID_ARG;
+    if (!mx_aligned(ep->bias, 4) || !mx_aligned(ep->row_scale, 4) || !mx_aligned(ep->col_scale, 4)) return GZ_ERR_MISALIGNED;
+    p.epi_flags = (ep->bias ? 1u : 0u) | (ep->row_scale ? 2u : 0u) | (ep->col_scale ? 4u : 0u);
+    p.act = (uint32_t)ep->activation;
+    p.bias = ep->bias;
+    p.row_scale = ep->row_scale;
+    p.col_scale = ep->col_scale;
+  }
+  p.alpha = *alpha;
+  p.beta = *beta;
+  p.c = *beta != 0.0f ? c : nullptr;
+  p.d = d;
+  p.c_vec_ok = (p.c && mx_aligned(c, 16) && (ds.ldc * size) % 16 == 0) ? 1u : 0u;
+  DeviceGuard guard(ds.device);
+  if (!guard.ok()) return GZ_ERR_CUDA;
+  return mx_launch(pl, &p, a, a_scales, b, b_scales, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+GZ_API gz_status gz_mx_gated_run(gz_mx_plan* pl, const void* a, const void* a_scales, const void* gate,
+                                 const void* gate_scales, const void* up, const void* up_scales, void* d,
+                                 void* d_scales, const float* alpha_gate, const float* alpha_up, int32_t activation,
+                                 float out_multiplier, void* stream) {
+  if (!pl || !a || !a_scales || !gate || !gate_scales || !up || !up_scales || !d || !alpha_gate || !alpha_up ||
+      !pl->pr.d.gated || activation < GZ_ACT_NONE || activation > GZ_ACT_SILU)
+    return GZ_ERR_INVALID_ARG;
+  const bool quantised = pl->pr.out_size == 0;
+  if (quantised != (d_scales != nullptr)) return GZ_ERR_INVALID_ARG;
+  if (quantised && (!(std::fabs(out_multiplier) <= 3.4028234e38f) || out_multiplier == 0.0f)) return GZ_ERR_INVALID_ARG;
+  if (!mx_aligned(a, 16) || !mx_aligned(a_scales, 16) || !mx_aligned(gate, 16) || !mx_aligned(gate_scales, 16) ||
+      !mx_aligned(up, 16) || !mx_aligned(up_scales, 16) || !mx_aligned(d, quantised ? 16 : pl->pr.out_size) ||
+      !mx_aligned(d_scales, 16))
+    return GZ_ERR_MISALIGNED;
+  gz::MxParams p = pl->base;
+  p.act = (uint32_t)activation;
+  p.alpha = *alpha_gate;
+  p.alpha_up = *alpha_up;
+  p.out_multiplier = out_multiplier;
+  p.d = d;
+  p.d_scales = static_cast<uint8_t*>(d_scales);
+  DeviceGuard guard(pl->pr.d.device);
+  if (!guard.ok()) return GZ_ERR_CUDA;
+  return mx_launch(pl, &p, a, a_scales, gate, gate_scales, up, up_scales, static_cast<cudaStream_t>(stream));
+}
+
+GZ_API gz_status gz_mx_last_device_status(gz_mx_plan* pl, void* stream_v, uint32_t detail[4]) {
+  if (!pl) return GZ_ERR_INVALID_ARG;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  DeviceGuard guard(pl->pr.d.device);
+  if (!guard.ok()) return GZ_ERR_CUDA;
+  uint32_t h[4] = {0, 0, 0, 0};
+  if (!cuda_ok(cudaStreamSynchronize(stream), "cudaStreamSynchronize") ||
+      !cuda_ok(cudaMemcpy(h, pl->status_dev, sizeof(h), cudaMemcpyDeviceToHost), "read status"))
+    return GZ_ERR_CUDA;
+  if (detail) std::memcpy(detail, h, sizeof(h));
+  if (h[0] == 0) return GZ_OK;
+  (void)cudaMemset(pl->status_dev, 0, sizeof(h));
+  return h[0] == gz::STORE_OUT_OF_BOUNDS ? GZ_ERR_DEBUG_CHECK : GZ_ERR_DEVICE_TIMEOUT;
+}
+
+}  // extern "C"
+#endif

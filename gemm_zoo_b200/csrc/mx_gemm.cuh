@@ -1,0 +1,797 @@
+// Product of two microscaled 4-bit matrices on the block-scaled tensor cores of sm_100a, and the
+// gated product of one with two (see include/gemmzoo/microscale.h for the operators):
+//
+//   D = act(alpha * row_scale * col_scale * A B^T + beta * C + bias)
+//   H = act(alpha * A G^T) * (alpha_up * A U^T)          (optionally quantised along its rows)
+//
+// The machinery is that of sm100_gemm.cuh (TMA producers, one MMA issuer, epilogue warps, bounded
+// waits) with a fourth ring operand: the scales.  A stage holds 256 elements of K: 128-byte-swizzled
+// rows of codes and, per 128 rows, 512-byte tiles of scales, which the MMA warp copies to tensor
+// memory (tcgen05.cp, four columns per tile, repeated for the four lane quadrants) right before the
+// tcgen05.mma that reads them.  Copies and MMAs of one thread execute in order, so the four scale slots
+// in tensor memory need no barrier of their own.
+//
+// Two tile families:
+//   pair     256 x 256 on a CTA pair (cta_group::2): A's rows on the 128-lane side, each CTA with its
+//            own 128 rows of A and its own 128 rows of B; scales of all 256 rows of B in both.  The
+//            gated product gives CTA 0 the gate's 128 rows and CTA 1 the up projection's: one MMA
+//            computes both halves and no operand is loaded twice.  Two fp32 accumulators of 256
+//            columns would fill tensor memory and leave no room for scales, so they overlap in 64
+//            columns: [0, 256) and [192, 448).  The epilogue reads the shared 64 columns first and
+//            the next tile's main loop starts while it works on the other 192.
+//   swapped  few rows of A: B's rows on the 128-lane side (128 features per tile), 16 to 128 rows of A
+//            on the narrow side, so every byte a stage loads is a useful byte of B.  The gated product
+//            keeps two row blocks per stage (gate and up).  Where tiles are fewer than SMs, a cluster
+//            of up to eight CTAs shares a tile's K range; the partial sums meet in shared memory
+//            (each CTA adds a share of the rows over distributed shared memory, in rank order), so there
+//            is no workspace, nothing to clear and one order of summation.
+#ifndef GZ_MX_GEMM_CUH
+#define GZ_MX_GEMM_CUH
+
+#include "mx_format.cuh"
+#include "sm100_gemm.cuh"
+
+namespace gz {
+
+// Output of a gated product: a gz_dtype, or one of these.
+constexpr uint32_t MX_OUT_FP4 = 16, MX_OUT_NVFP4 = 17;
+
+struct MxMaps {
+  CUtensorMap wide, wide_scales;      // the operand on the 128-lane side
+  CUtensorMap narrow, narrow_scales;  // the other one
+  CUtensorMap up, up_scales;          // gated: the up projection (the gate is `wide` of a swapped tile, `narrow` of a pair)
+  CUtensorMap d;
+};
+
+struct MxParams {
+  TileGrid grid;  // tiles_m along the 128-lane side
+  uint32_t m, n;  // rows and columns of the output
+  uint32_t k_blocks;
+  uint32_t split;  // swapped tiles: CTAs (one cluster) that share a tile's K range
+  uint32_t idesc;
+  uint32_t out_type;
+  uint32_t out_tma, c_vec_ok;
+  uint32_t test_flags;
+  uint32_t epi_flags, act;  // bit 0 bias, 1 row_scale, 2 col_scale
+  float alpha, alpha_up, beta, out_multiplier;
+  const float* bias;
+  const float* row_scale;
+  const float* col_scale;
+  const void* c;
+  void* d;
+  uint8_t* d_scales;
+  int64_t ldc, ldd;   // elements (a quantised output: bytes)
+  int64_t d_groups;   // quantised output: scale tiles per 128 rows
+  uint32_t* status;
+  uint64_t wait_limit_ns;
+};
+
+template <bool NV_, int BN_, bool PAIR_, bool GATED_>
+struct MxCfg {
+  static constexpr bool NV = NV_, PAIR = PAIR_, GATED = GATED_;
+  static constexpr int BN = BN_;
+  static constexpr int CTAS = PAIR ? 2 : 1;
+  static constexpr int MB = (GATED && !PAIR) ? 2 : 1;  // 128-row blocks on the wide side per CTA
+  static constexpr int TILES_K = NV ? 4 : 2;           // scale tiles per stage and 128 rows
+  static constexpr int NRB = BN > 128 ? 2 : 1;         // scale row groups of the narrow side
+  static constexpr int W_BYTES = MB * 128 * 128;
+  static constexpr int N_BYTES = (BN / CTAS) * 128;
+  static constexpr int WS_BYTES = MB * TILES_K * 512;
+  static constexpr int NS_BYTES = NRB * TILES_K * 512;
+  static constexpr int STAGE_BYTES = W_BYTES + N_BYTES + WS_BYTES + NS_BYTES;
+  static constexpr int EPI_WARPS = PAIR ? 8 : 4;
+  static constexpr int STAGING_BYTES = PAIR ? EPI_WARPS * 4096 : 0;
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int MAX_STAGES = (232448 - 1024 - STAGING_BYTES - BAR_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = MAX_STAGES < 12 ? MAX_STAGES : 12;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + RING_BYTES + STAGING_BYTES + BAR_BYTES;
+  static constexpr int THREADS = 96 + 32 * EPI_WARPS;
+  // Tensor memory: accumulators, then four 16-column scale slots.
+  static constexpr int NBUF = PAIR ? 1 : (2 * MB * BN + 64 <= 512 ? 2 : 1);  // accumulator barriers
+  static constexpr int ACC_COLS = PAIR ? 448 : NBUF * MB * BN;
+  static constexpr int SLOT_COLS = 16;
+  static constexpr int TMEM_COLS = ACC_COLS + 64 <= 128 ? 128 : ACC_COLS + 64 <= 256 ? 256 : 512;
+  static_assert(ACC_COLS % 16 == 0 && ACC_COLS + 64 <= TMEM_COLS, "tensor memory");
+  static_assert(PAIR ? BN == 256 : (BN >= 16 && BN <= 128 && BN % 16 == 0), "tile shapes");
+  static_assert(STAGE_BYTES % 1024 == 0 && STAGES >= 4, "ring");
+  static_assert(PAIR || MB * BN * 128 * 4 <= RING_BYTES, "partial sums meet in the ring");
+  static_assert(8 * (2 * STAGES + 5) + 16 <= BAR_BYTES, "barriers");
+};
+
+namespace detail {
+
+#if defined(GZ_BOUNDS_CHECK)
+static __device__ __noinline__ bool mx_store_in_bounds(const MxParams& p, uint32_t row, uint32_t col, uint32_t ncols,
+                                                       uint32_t rows, uint32_t cols) {
+  if (row < rows && col < cols && ncols <= cols - col) return true;
+  if (atomicCAS(p.status, 0u, STORE_OUT_OF_BOUNDS) == 0u) {
+    p.status[1] = blockIdx.x;
+    p.status[2] = row;
+    p.status[3] = col;
+    __threadfence();
+  }
+  return false;
+}
+#define GZ_MX_STORE_OK(p, row, col, ncols, rows, cols) detail::mx_store_in_bounds(p, row, col, ncols, rows, cols)
+#else
+#define GZ_MX_STORE_OK(p, row, col, ncols, rows, cols) true
+#endif
+
+// One activation's code per pass.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&f)[N], uint32_t act) {
+  switch (act) {
+    case 1:
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = activate(f[i], 1);
+      break;
+    case 2:
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = activate(f[i], 2);
+      break;
+    case 3:
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = activate(f[i], 3);
+      break;
+    case 4:
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = activate(f[i], 4);
+      break;
+    default: break;
+  }
+}
+
+__device__ __forceinline__ float mx_load_c(const MxParams& p, int64_t at) {
+  switch (p.out_type) {
+    case 0: return __half2float(static_cast<const __half*>(p.c)[at]);
+    case 1: return __bfloat162float(static_cast<const __nv_bfloat16*>(p.c)[at]);
+    default: return static_cast<const float*>(p.c)[at];
+  }
+}
+__device__ __forceinline__ void mx_store(const MxParams& p, int64_t at, float v) {
+  switch (p.out_type) {
+    case 0: static_cast<__half*>(p.d)[at] = __float2half_rn(v); break;
+    case 1: static_cast<__nv_bfloat16*>(p.d)[at] = __float2bfloat16_rn(v); break;
+    default: static_cast<float*>(p.d)[at] = v;
+  }
+}
+
+// The optional terms on 32 columns of one row (the pair tile).
+__device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], uint32_t row, uint32_t col0,
+                                             uint32_t lane) {
+  const bool row_ok = row < p.m;
+  const uint32_t ncols = p.n - col0 < 32u ? p.n - col0 : 32u;
+  const bool col_ok = lane < ncols;
+  if (p.epi_flags & 2u) {
+    const float rs = row_ok ? __ldg(p.row_scale + row) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] *= rs;
+  }
+  if (p.epi_flags & 4u) {
+    const float mine = col_ok ? __ldg(p.col_scale + col0 + lane) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] *= __shfl_sync(0xFFFFFFFFu, mine, i);
+  }
+  if (p.beta != 0.0f && row_ok) {
+    const int64_t at = static_cast<int64_t>(row) * p.ldc + col0;
+    if (ncols == 32u && p.c_vec_ok) {
+      if (p.out_type == 2u) {
+        const float4* c4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.c) + at);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 c = c4[q];
+          f[4 * q] = fmaf(p.beta, c.x, f[4 * q]);
+          f[4 * q + 1] = fmaf(p.beta, c.y, f[4 * q + 1]);
+          f[4 * q + 2] = fmaf(p.beta, c.z, f[4 * q + 2]);
+          f[4 * q + 3] = fmaf(p.beta, c.w, f[4 * q + 3]);
+        }
+      } else {
+        const uint4* c4 = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c) + at);
+        uint32_t w[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint4 c = c4[q];
+          w[4 * q] = c.x;
+          w[4 * q + 1] = c.y;
+          w[4 * q + 2] = c.z;
+          w[4 * q + 3] = c.w;
+        }
+        const bool half_in = p.out_type == 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 c = half_in ? unpack2<__half>(w[i]) : unpack2<__nv_bfloat16>(w[i]);
+          f[2 * i] = fmaf(p.beta, c.x, f[2 * i]);
+          f[2 * i + 1] = fmaf(p.beta, c.y, f[2 * i + 1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (static_cast<uint32_t>(i) < ncols) f[i] = fmaf(p.beta, mx_load_c(p, at + i), f[i]);
+    }
+  }
+  if (p.epi_flags & 1u) {
+    const float mine = col_ok ? __ldg(p.bias + col0 + lane) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] += __shfl_sync(0xFFFFFFFFu, mine, i);
+  }
+  activate_all(f, p.act);
+}
+
+// 32 rows x 32 columns (lane = row) to the output through the warp's 4 KB of staging: a TMA store of a
+// swizzled box, or, where TMA cannot describe D, whole row pieces with plain stores.  `turn` alternates
+// the two halves of the staging for 16-bit outputs.
+__device__ __forceinline__ void mx_store_box(const MxParams& p, const void* tm_d, uint32_t stg, uint32_t lane,
+                                             const float (&f)[32], uint32_t row0, uint32_t col0, uint32_t& turn) {
+  const bool wide = p.out_type == 2u;
+  const uint32_t box = wide ? stg : stg + (turn & 1u) * 2048u;
+  if (p.out_tma) {
+    if (lane == 0) {
+      if (wide) ptx::bulk_wait_group_read<0>();
+      else ptx::bulk_wait_group_read<1>();
+    }
+  }
+  __syncwarp();
+  if (wide) {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128u + ((j ^ (lane & 7u)) << 4)),
+                   "f"(f[4 * j]), "f"(f[4 * j + 1]), "f"(f[4 * j + 2]), "f"(f[4 * j + 3])
+                   : "memory");
+  } else {
+    uint32_t w[16];
+    if (p.out_type == 0u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack2<__half>(f[2 * i], f[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack2<__nv_bfloat16>(f[2 * i], f[2 * i + 1]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 64u + ((j ^ ((lane >> 1) & 3u)) << 4)),
+                   "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                   : "memory");
+  }
+  if (p.out_tma) {
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      ptx::tma_store_3d(tm_d, box, static_cast<int32_t>(col0), static_cast<int32_t>(row0), 0);
+      ptx::bulk_commit_group();
+    }
+  } else {
+    __syncwarp();
+    const uint32_t rows = p.m - row0 < 32u ? p.m - row0 : 32u;
+    const bool ok = lane < p.n - col0;
+    for (uint32_t r = 0; r < rows; ++r) {
+      const int64_t at = static_cast<int64_t>(row0 + r) * p.ldd + col0 + lane;
+      if (!ok || !GZ_MX_STORE_OK(p, row0 + r, col0 + lane, 1u, p.m, p.n)) continue;
+      if (wide) {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(box + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u) : "memory");
+        static_cast<uint32_t*>(p.d)[at] = v;
+      } else {
+        uint16_t v;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(box + r * 64u + (((lane >> 3) ^ ((r >> 1) & 3u)) << 4) + (lane & 7u) * 2u) : "memory");
+        static_cast<uint16_t*>(p.d)[at] = v;
+      }
+    }
+    __syncwarp();
+  }
+  ++turn;
+}
+
+// 32 columns of one row, quantised: the codes and the one or two scales (pair tile; lane = row).
+template <bool NV>
+__device__ __forceinline__ void mx_store_quantized(const MxParams& p, const float (&f)[32], uint32_t row, uint32_t col0) {
+  constexpr int BLOCK = mx::Format<NV>::BLOCK;
+  const bool row_ok = row < p.m;
+  uint32_t codes[4];
+#pragma unroll
+  for (int b = 0; b < 32 / BLOCK; ++b) {
+    float v[BLOCK];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < BLOCK; ++i) {
+      v[i] = col0 + b * BLOCK + i < p.n ? f[b * BLOCK + i] * p.out_multiplier : 0.0f;
+      amax = mx::amax_nan(amax, v[i]);
+    }
+    const mx::Scale s = mx::block_scale<NV>(amax);
+#pragma unroll
+    for (int i = 0; i < BLOCK / 8; ++i) {
+      float* x = &v[i * 8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = mx::in_code_units<NV>(x[j], s);
+      const uint32_t c = mx::pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+      codes[b * (BLOCK / 8) + i] = s.byte == mx::Format<NV>::NAN_SCALE ? 0u : c;
+    }
+    const int64_t block = static_cast<int64_t>(col0) / BLOCK + b;
+    if (block < 4 * p.d_groups)  // rows up to the next multiple of 128 exist in the scale array
+      p.d_scales[mx::scale_word(row, block >> 2, p.d_groups) + (block & 3)] = static_cast<uint8_t>(row_ok ? s.byte : 0u);
+  }
+  if (row_ok && col0 < p.n && GZ_MX_STORE_OK(p, row, col0, 1u, p.m, p.n))
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.d) + static_cast<int64_t>(row) * p.ldd + col0 / 2) =
+        make_uint4(codes[0], codes[1], codes[2], codes[3]);
+}
+
+// One output row of a swapped tile, quantised: the warp's 32 lanes are 32 consecutive columns.
+template <bool NV>
+__device__ __forceinline__ void mx_store_quantized_lane(const MxParams& p, float h, uint32_t row, uint32_t col0,
+                                                        uint32_t lane) {
+  const float v = col0 + lane < p.n ? h * p.out_multiplier : 0.0f;
+  const uint32_t mask = NV ? (lane < 16u ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
+  // as integers the magnitudes order like the numbers, with NaN above infinity
+  const uint32_t top = __reduce_max_sync(mask, __float_as_uint(v) & 0x7FFFFFFFu);
+  const mx::Scale s = mx::block_scale<NV>(__uint_as_float(top));
+  uint32_t word = s.byte == mx::Format<NV>::NAN_SCALE ? 0u : mx::pack1(mx::in_code_units<NV>(v, s)) << (4u * (lane & 7u));
+#pragma unroll
+  for (int d = 1; d < 8; d *= 2) word |= __shfl_xor_sync(0xFFFFFFFFu, word, d);
+  if ((lane & 7u) == 0u && col0 < p.n && GZ_MX_STORE_OK(p, row, col0, 1u, p.m, p.n))
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.d) + static_cast<int64_t>(row) * p.ldd + (col0 + lane) / 2) = word;
+  constexpr uint32_t BLOCK = mx::Format<NV>::BLOCK;
+  const int64_t block = (col0 + lane) / BLOCK;
+  if (lane % BLOCK == 0u && block < 4 * p.d_groups)
+    p.d_scales[mx::scale_word(row, block >> 2, p.d_groups) + (block & 3)] = static_cast<uint8_t>(s.byte);
+}
+
+}  // namespace detail
+
+// Finish up to N output rows row0, row0 + step, ... of a swapped tile: the lane is column col0 + lane,
+// f (and u) are the accumulators.  All 32 lanes take part.
+template <class Cfg, int N>
+__device__ __forceinline__ void mx_finish_rows(const MxParams& p, float (&f)[N], float (&u)[N], uint32_t row0,
+                                               uint32_t step, uint32_t count, uint32_t col0, uint32_t lane) {
+  const uint32_t col = col0 + lane;
+  const bool col_ok = col < p.n;
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] *= p.alpha;
+  if constexpr (Cfg::GATED) {
+    detail::activate_all(f, p.act);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] *= p.alpha_up * u[i];
+    if (p.out_type >= MX_OUT_FP4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (static_cast<uint32_t>(i) >= count) break;
+        if (p.out_type == MX_OUT_FP4) detail::mx_store_quantized_lane<false>(p, f[i], row0 + i * step, col0, lane);
+        else detail::mx_store_quantized_lane<true>(p, f[i], row0 + i * step, col0, lane);
+      }
+      return;
+    }
+  } else {
+    if (p.epi_flags & 2u) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (static_cast<uint32_t>(i) < count) f[i] *= __ldg(p.row_scale + row0 + i * step);
+    }
+    if (p.epi_flags & 4u) {
+      const float cs = col_ok ? __ldg(p.col_scale + col) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] *= cs;
+    }
+    if (p.beta != 0.0f && col_ok) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (static_cast<uint32_t>(i) < count)
+          f[i] = fmaf(p.beta, detail::mx_load_c(p, static_cast<int64_t>(row0 + i * step) * p.ldc + col), f[i]);
+    }
+    if (p.epi_flags & 1u) {
+      const float b = col_ok ? __ldg(p.bias + col) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] += b;
+    }
+    detail::activate_all(f, p.act);
+  }
+  if (!col_ok) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (static_cast<uint32_t>(i) < count && GZ_MX_STORE_OK(p, row0 + i * step, col, 1u, p.m, p.n))
+      detail::mx_store(p, static_cast<int64_t>(row0 + i * step) * p.ldd + col, f[i]);
+}
+
+// Quantised output of a swapped tile: the scale rows from m up to the next multiple of 128 are zero.
+// `thread` (0..127) takes row 128 * group + thread of the tile's one (e8m0) or two (e4m3) scale tiles.
+__device__ __forceinline__ void mx_clear_scale_rows(const MxParams& p, uint32_t tm, uint32_t group, uint32_t thread) {
+  if (p.out_type < MX_OUT_FP4) return;
+  const uint32_t row = group * 128u + thread;
+  if (row < p.m) return;
+  const uint32_t words = p.out_type == MX_OUT_NVFP4 ? 2u : 1u;
+  for (uint32_t w = 0; w < words; ++w) {
+    const int64_t g = static_cast<int64_t>(tm) * words + w;
+    if (g < p.d_groups) *reinterpret_cast<uint32_t*>(p.d_scales + mx::scale_word(row, g, p.d_groups)) = 0u;
+  }
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
+  constexpr int CTAS = Cfg::CTAS, STAGES = Cfg::STAGES, BN = Cfg::BN, MB = Cfg::MB, NBUF = Cfg::NBUF;
+  constexpr bool NV = Cfg::NV, PAIR = Cfg::PAIR, GATED = Cfg::GATED;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - raw_addr);
+  const uint32_t staging_base = base + Cfg::RING_BYTES;
+  const uint32_t bars = staging_base + Cfg::STAGING_BYTES;
+  auto full_bar = [&](uint32_t s) { return bars + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bars + 8u * (STAGES + s); };
+  auto acc_full_bar = [&](uint32_t b) { return bars + 8u * (2 * STAGES + b); };
+  auto acc_empty_bar = [&](uint32_t b) { return bars + 8u * (2 * STAGES + 2 + b); };
+  const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4);
+  uint32_t* const tmem_slot =
+      reinterpret_cast<uint32_t*>(smem + Cfg::RING_BYTES + Cfg::STAGING_BYTES + 8 * (2 * STAGES + 5));
+  uint32_t* const abort_flag = tmem_slot + 1;
+
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t rank = ptx::cluster_ctarank();  // of the pair, or of the cluster that shares a K range
+  const uint32_t cluster = ptx::cluster_id_x(), num_clusters = ptx::num_clusters_x();
+  const detail::Abort ab{abort_flag, p.status, p.wait_limit_ns};
+
+  // ------------------------------------------------------------ set-up (as in sm100_gemm.cuh)
+  if (warp == 0) {
+    if (lane == 31u) ptx::prefetch_tensormap(&maps.wide);
+    if (lane == 30u) ptx::prefetch_tensormap(&maps.wide_scales);
+    if (lane == 29u && p.out_tma) ptx::prefetch_tensormap(&maps.d);
+    for (uint32_t s = lane; s < STAGES; s += 32u) {
+      ptx::mbar_init(full_bar(s), 2);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    if (lane < 2u) {
+      ptx::mbar_init(acc_full_bar(lane), 1);
+      ptx::mbar_init(acc_empty_bar(lane), Cfg::EPI_WARPS * CTAS);
+    }
+    if (lane == 2u) {
+      ptx::mbar_init(drain_bar, 1);
+      *abort_flag = 0u;
+    }
+    ptx::fence_mbar_init_cluster();
+    __syncwarp();
+    ptx::named_barrier_arrive(2, 64);
+    ptx::named_barrier_arrive(3, Cfg::THREADS - 32);
+    if constexpr (CTAS == 2) ptx::cluster_arrive_release();
+  } else if (warp == 6) {
+    if (lane == 0) ptx::prefetch_tensormap(&maps.narrow);
+    if (lane == 1) ptx::prefetch_tensormap(&maps.narrow_scales);
+    if (GATED && lane == 2) ptx::prefetch_tensormap(&maps.up);
+    if (GATED && lane == 3) ptx::prefetch_tensormap(&maps.up_scales);
+    if constexpr (CTAS == 2) ptx::cluster_arrive_release();
+    ptx::named_barrier_sync(2, 64);
+  } else {
+    if constexpr (CTAS == 2) ptx::cluster_arrive_release();
+    if (warp == 1) {
+      ptx::tmem_alloc<CTAS>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
+      ptx::tmem_relinquish<CTAS>();
+    }
+    ptx::tc_fence_before_sync();
+    ptx::named_barrier_sync(3, Cfg::THREADS - 32);
+    ptx::tc_fence_after_sync();
+  }
+  if constexpr (CTAS == 2) ptx::cluster_wait_acquire();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  ptx::grid_launch_dependents();
+
+  // The tiles of this cluster and the K blocks of each that are this CTA's.
+  uint32_t kb_lo = 0, kb_hi = p.k_blocks;
+  if constexpr (!PAIR) {
+    if (p.split > 1u) {
+      kb_lo = static_cast<uint32_t>(static_cast<uint64_t>(rank) * p.k_blocks / p.split);
+      kb_hi = static_cast<uint32_t>(static_cast<uint64_t>(rank + 1u) * p.k_blocks / p.split);
+    }
+  }
+
+  if (warp == 0 || warp == 6) {
+    // ---------------------------------------------------------- TMA producers
+    // Warp 0: the wide operand and its scales; warp 6: the narrow one.
+    const bool is_narrow = warp == 6;
+    const uint32_t my_bytes = is_narrow ? Cfg::N_BYTES + Cfg::NS_BYTES : Cfg::W_BYTES + Cfg::WS_BYTES;
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    ptx::grid_dependency_wait();
+    for (uint32_t t = cluster; ok && t < p.grid.num_tiles; t += num_clusters) {
+      uint32_t tm, tn;
+      tile_coords(p.grid, t, tm, tn);
+      const int32_t wide_rb = static_cast<int32_t>(PAIR ? tm * 2u + rank : tm);
+      for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
+        ok = __all_sync(0xFFFFFFFFu, detail::wait(empty_bar(stage), phase ^ 1u, ab, WAIT_PRODUCER_EMPTY, t, kb));
+        if (!ok) break;
+        if (ptx::elect_one()) {
+          const uint32_t dst = base + stage * Cfg::STAGE_BYTES;
+          const int32_t kx = static_cast<int32_t>(kb * 128u);
+          const int32_t kt = static_cast<int32_t>(kb * Cfg::TILES_K);
+          uint32_t fb = full_bar(stage);
+          if constexpr (CTAS == 1) {
+            ptx::mbar_arrive_expect_tx(fb, my_bytes);
+          } else {
+            if (rank == 0) ptx::mbar_arrive_expect_tx(fb, 2u * my_bytes);
+            fb = ptx::mapa(fb, 0);
+          }
+          auto load = [&](uint32_t to, const void* map, int32_t c0, int32_t c1, int32_t c2) {
+            if constexpr (CTAS == 1) ptx::tma_load_3d(to, map, c0, c1, c2, fb);
+            else ptx::tma_load_3d_pair(to, map, c0, c1, c2, fb);
+          };
+          const uint32_t ws = dst + Cfg::W_BYTES + Cfg::N_BYTES, ns = ws + Cfg::WS_BYTES;
+          if (!is_narrow) {
+            load(dst, &maps.wide, kx, wide_rb * 128, 0);
+            load(ws, &maps.wide_scales, 0, kt, wide_rb);
+            if constexpr (MB == 2) {
+              load(dst + 128u * 128u, &maps.up, kx, wide_rb * 128, 0);
+              load(ws + Cfg::TILES_K * 512u, &maps.up_scales, 0, kt, wide_rb);
+            }
+          } else if constexpr (PAIR) {
+            const int32_t rb0 = static_cast<int32_t>(GATED ? tn : tn * 2u);
+            const CUtensorMap* const second_scales = GATED ? &maps.up_scales : &maps.narrow_scales;
+            const int32_t rb1 = GATED ? rb0 : rb0 + 1;
+            load(dst + Cfg::W_BYTES, (GATED && rank == 1u) ? &maps.up : &maps.narrow, kx,
+                 (rank == 0u ? rb0 : rb1) * 128, 0);
+            load(ns, &maps.narrow_scales, 0, kt, rb0);
+            load(ns + Cfg::TILES_K * 512u, second_scales, 0, kt, rb1);
+          } else {
+            load(dst + Cfg::W_BYTES, &maps.narrow, kx, static_cast<int32_t>(tn * BN), 0);
+            load(ns, &maps.narrow_scales, 0, kt, static_cast<int32_t>(tn * BN / 128u));
+          }
+        }
+        __syncwarp();
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok && rank == 0 && lane == 0) {
+      // Aborting: give loads already issued a bounded chance to land (see sm100_gemm.cuh).
+      const uint64_t t0 = ptx::globaltimer_ns();
+      for (uint32_t i = 0; i < STAGES; ++i) {
+        const uint32_t s = (stage + STAGES - 1u - i) % STAGES;
+        const uint32_t ph = (s < stage) ? phase : (phase ^ 1u);
+        while (!ptx::mbar_try_wait(full_bar(s), ph)) {
+          if (ptx::globaltimer_ns() - t0 > 2000000ull) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    ptx::grid_dependency_wait();
+    if (!PAIR || rank == 0) {
+      uint32_t stage = 0, phase = 0, it = 0, slot = 0;
+      bool ok = true, issued = false;
+      // Shared-memory descriptors: codes in 128-byte-swizzled rows (8 rows = 1024 bytes); scales as
+      // 32 rows of 16 bytes, 8 rows = 128 bytes, unswizzled.
+      const uint64_t code_hi = static_cast<uint64_t>((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | (1u << 16);
+      const uint64_t scale_hi = static_cast<uint64_t>((128u >> 4) | (1u << 14)) << 32 | ((128u >> 4) << 16);
+      for (uint32_t t = cluster; ok && t < p.grid.num_tiles; t += num_clusters, ++it) {
+        const uint32_t buf = it % NBUF;
+        ok = __all_sync(0xFFFFFFFFu, detail::wait(acc_empty_bar(buf), ((it / NBUF) & 1u) ^ 1u, ab, WAIT_MMA_TMEM_EMPTY, t, 0));
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + (PAIR ? (it & 1u) * 192u : buf * (MB * BN));
+        uint32_t narrow_off = 0;  // scale columns of the narrow tile's first row within its group of 128
+        if constexpr (!PAIR && BN < 128) {
+          uint32_t tm, tn;
+          tile_coords(p.grid, t, tm, tn);
+          narrow_off = (tn * BN % 128u) / 32u;
+        }
+        for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
+          ok = __all_sync(0xFFFFFFFFu, detail::wait(full_bar(stage), phase, ab, WAIT_MMA_FULL, t, kb));
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          if (ptx::elect_one()) {
+            const uint32_t st = base + stage * Cfg::STAGE_BYTES;
+            const uint32_t ws = st + Cfg::W_BYTES + Cfg::N_BYTES, ns = ws + Cfg::WS_BYTES;
+            const uint64_t wd = code_hi | ((st >> 4) & 0x3FFFu), nd = code_hi | (((st + Cfg::W_BYTES) >> 4) & 0x3FFFu);
+#pragma unroll
+            for (uint32_t a = 0; a < static_cast<uint32_t>(Cfg::TILES_K); ++a) {
+              const uint32_t sf = tmem_base + Cfg::ACC_COLS + ((slot + a) & 3u) * Cfg::SLOT_COLS;
+#pragma unroll
+              for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb)
+                ptx::tmem_copy_scales<CTAS>(sf + mb * 4u, scale_hi | (((ws + (mb * Cfg::TILES_K + a) * 512u) >> 4) & 0x3FFFu));
+#pragma unroll
+              for (uint32_t rb = 0; rb < static_cast<uint32_t>(Cfg::NRB); ++rb)
+                ptx::tmem_copy_scales<CTAS>(sf + 8u + rb * 4u, scale_hi | (((ns + (rb * Cfg::TILES_K + a) * 512u) >> 4) & 0x3FFFu));
+              constexpr uint32_t STEPS = 4 / Cfg::TILES_K;  // MMAs per scale tile
+#pragma unroll
+              for (uint32_t j = 0; j < STEPS; ++j) {
+                // which of the four scales of a row this step starts at (two per step for e8m0)
+                const uint32_t idesc = p.idesc | (j * 2u) << 4 | (j * 2u) << 29;
+                const uint32_t step = a * STEPS + j;
+#pragma unroll
+                for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb)
+                  ptx::umma_mx<NV, CTAS>(d_tmem + mb * BN, wd + step * 2u + mb * ((128u * 128u) >> 4), nd + step * 2u,
+                                         idesc, sf + mb * 4u, sf + 8u + narrow_off, (kb != kb_lo || step != 0u) ? 1u : 0u);
+              }
+            }
+            ptx::tc_commit<CTAS>(empty_bar(stage));
+            if constexpr (CTAS == 2) ptx::tc_commit<CTAS>(ptx::mapa(empty_bar(stage), 1));
+          }
+          __syncwarp();
+          issued = true;
+          slot = (slot + Cfg::TILES_K) & 3u;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (!(p.test_flags & 1u) && ptx::elect_one()) {
+          ptx::tc_commit<CTAS>(acc_full_bar(buf));
+          if constexpr (CTAS == 2) ptx::tc_commit<CTAS>(ptx::mapa(acc_full_bar(buf), 1));
+        }
+        __syncwarp();
+      }
+      if ((!ok || (p.test_flags & 1u)) && issued && lane == 0) {
+        ptx::tc_commit<CTAS>(drain_bar);
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (!ptx::mbar_try_wait(drain_bar, 0)) {
+          if (ptx::globaltimer_ns() - t0 > 2000000ull) break;
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue
+    ptx::grid_dependency_wait();
+    const uint32_t quad = warp & 3u;
+    const uint32_t lanes = tmem_base + ((quad * 32u) << 16);
+    uint32_t it = 0;
+    if constexpr (PAIR) {
+      const uint32_t half = warp >= 7u ? 1u : 0u;
+      const uint32_t stg = staging_base + (half * 4u + quad) * 4096u;
+      const uint32_t release = ptx::mapa(acc_empty_bar(0), 0);
+      uint32_t turn = 0;
+      for (uint32_t t = cluster; t < p.grid.num_tiles; t += num_clusters, ++it) {
+        uint32_t tm, tn;
+        tile_coords(p.grid, t, tm, tn);
+        const uint32_t row0 = tm * 256u + rank * 128u + quad * 32u;
+        if (!detail::wait(acc_full_bar(0), it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t acc = lanes + (it & 1u) * 192u;
+        constexpr uint32_t GROUPS = GATED ? 2u : 4u;  // of 64 columns; this warp's half of each is 32 wide
+#pragma unroll 1
+        for (uint32_t s = 0; s < GROUPS; ++s) {
+          // the group that the next tile's accumulator overlaps comes first
+          const uint32_t g = (it & 1u) ? s : (s + GROUPS - 1u) % GROUPS;
+          const uint32_t off = g * 64u + half * 32u;
+          uint32_t x[32], y[32];
+          ptx::tmem_ld_32x32(acc + off, x);
+          if constexpr (GATED) ptx::tmem_ld_32x32(acc + 128u + off, y);
+          ptx::tmem_wait_ld();
+          if (s == 0) {
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(release);
+          }
+          const uint32_t col0 = tn * (GATED ? 128u : 256u) + off;
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = p.alpha * __uint_as_float(x[i]);
+          if constexpr (GATED) {
+            detail::activate_all(f, p.act);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] *= p.alpha_up * __uint_as_float(y[i]);
+            if (p.out_type >= MX_OUT_FP4) {
+              if (row0 < ((p.m + 127u) & ~127u)) {
+                if (p.out_type == MX_OUT_FP4) detail::mx_store_quantized<false>(p, f, row0 + lane, col0);
+                else detail::mx_store_quantized<true>(p, f, row0 + lane, col0);
+              }
+              continue;
+            }
+            if (row0 >= p.m || col0 >= p.n) continue;
+          } else {
+            if (row0 >= p.m || col0 >= p.n) continue;
+            if (p.epi_flags != 0u || p.beta != 0.0f || p.act != 0u) detail::mx_row_terms(p, f, row0 + lane, col0, lane);
+          }
+          detail::mx_store_box(p, &maps.d, stg, lane, f, row0, col0, turn);
+        }
+        // the barrier counts one release per tile, made above; the rest of this tile's columns are read
+        // before the next tile's release, which is what the tile after that waits for
+        ptx::tc_fence_before_sync();
+      }
+      if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
+    } else {
+      const uint32_t feature_in_tile = quad * 32u + lane;
+      for (uint32_t t = cluster; t < p.grid.num_tiles; t += num_clusters, ++it) {
+        uint32_t tm, tn;
+        tile_coords(p.grid, t, tm, tn);
+        const uint32_t buf = it % NBUF;
+        if (!detail::wait(acc_full_bar(buf), (it / NBUF) & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t acc = lanes + buf * (MB * BN);
+        const uint32_t token0 = tn * BN;
+        const uint32_t tokens = p.m - token0 < static_cast<uint32_t>(BN) ? p.m - token0 : static_cast<uint32_t>(BN);
+#pragma unroll 1
+        for (uint32_t sl = 0; sl * 16u < tokens; ++sl) {
+          uint32_t x[16], y[16];
+          ptx::tmem_ld_32x16(acc + sl * 16u, x);
+          if constexpr (GATED) ptx::tmem_ld_32x16(acc + BN + sl * 16u, y);
+          ptx::tmem_wait_ld();
+          if (p.split > 1u) {
+            // Park the partial sums: [operand][row of A][128 features].
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+              const uint32_t at = base + ((sl * 16u + i) * 128u + feature_in_tile) * 4u;
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x[i]) : "memory");
+              if constexpr (GATED)
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + BN * 512u), "r"(y[i]) : "memory");
+            }
+          } else {
+            float f[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(x[i]);
+            float u[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = GATED ? __uint_as_float(y[i]) : 0.0f;
+            const uint32_t count = tokens - sl * 16u < 16u ? tokens - sl * 16u : 16u;
+            mx_finish_rows<Cfg, 16>(p, f, u, token0 + sl * 16u, 1u, count, tm * 128u + quad * 32u, lane);
+          }
+        }
+        if (p.split <= 1u) {
+          if constexpr (GATED) mx_clear_scale_rows(p, tm, token0 / 128u, (warp & 3u) * 32u + lane);
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(acc_empty_bar(buf));
+        }
+      }
+    }
+  }
+
+  // -------------------------------------------------------------- shared K range: add the partial sums
+  if constexpr (!PAIR) {
+    if (p.split > 1u) {
+      __syncwarp();
+      ptx::cluster_arrive_release();
+      ptx::cluster_wait_acquire();
+      const bool epilogue = warp >= 2u && warp != 6u;
+      if (epilogue && cluster < p.grid.num_tiles && !detail::aborted(ab)) {
+        uint32_t tm, tn;
+        tile_coords(p.grid, cluster, tm, tn);
+        const uint32_t quad = warp & 3u;
+        const uint32_t token0 = tn * BN;
+        const uint32_t tokens = p.m - token0 < static_cast<uint32_t>(BN) ? p.m - token0 : static_cast<uint32_t>(BN);
+        const uint32_t mine = base + (quad * 32u + lane) * 4u;
+        // rows rank, rank + split, ... of the tile, four at a time
+        for (uint32_t r = rank; r < tokens; r += 4u * p.split) {
+          float f[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint32_t count = (tokens - r + p.split - 1u) / p.split < 4u ? (tokens - r + p.split - 1u) / p.split : 4u;
+          for (uint32_t q = 0; q < p.split; ++q) {
+            const uint32_t peer = ptx::mapa(mine, q);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+              if (i >= count) break;
+              const uint32_t at = peer + (r + i * p.split) * 512u;
+              f[i] += ptx::ld_cluster_f32(at);
+              if constexpr (GATED) u[i] += ptx::ld_cluster_f32(at + BN * 512u);
+            }
+          }
+          mx_finish_rows<Cfg, 4>(p, f, u, token0 + r, p.split, count, tm * 128u + quad * 32u, lane);
+        }
+        if (GATED && rank == 0) mx_clear_scale_rows(p, tm, token0 / 128u, (warp & 3u) * 32u + lane);
+      }
+      __syncwarp();
+      ptx::cluster_arrive_release();  // nobody leaves while a peer may still read its partial sums
+      ptx::cluster_wait_acquire();
+    }
+  }
+
+  // -------------------------------------------------------------- teardown (as in sm100_gemm.cuh)
+  __syncwarp();
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::grid_dependency_wait();
+  if (detail::aborted(ab)) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 100000ull) __nanosleep(1000);
+  }
+  if constexpr (CTAS == 2) {
+    ptx::cluster_arrive_release();
+    ptx::cluster_wait_acquire();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc<CTAS>(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace gz
+#endif

@@ -301,6 +301,49 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t 
 #undef GZ_UMMA
 }
 
+// Block-scaled 4-bit product: D[tmem] (+)= (A * scale A) * (B * scale B), K = 64 per instruction; the
+// scales lie in tensor memory.  NV: e4m3 scales per 16 elements, otherwise e8m0 per 32.
+template <bool NV, int CTAS>
+__device__ __forceinline__ void umma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t a_scale, uint32_t b_scale, uint32_t accumulate) {
+#define GZ_UMMA_MX(GROUP, KINDSTR, VEC)                                                                  \
+  asm volatile(                                                                                          \
+      "{\n\t"                                                                                            \
+      ".reg .pred p;\n\t"                                                                                \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                        \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KINDSTR ".block_scale.scale_vec::" VEC                   \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t"                                                            \
+      "}"                                                                                                \
+      :                                                                                                  \
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)   \
+      : "memory")
+  if constexpr (CTAS == 1) {
+    if constexpr (NV) GZ_UMMA_MX("1", "mxf4nvf4", "4X");
+    else GZ_UMMA_MX("1", "mxf4", "2X");
+  } else {
+    if constexpr (NV) GZ_UMMA_MX("2", "mxf4nvf4", "4X");
+    else GZ_UMMA_MX("2", "mxf4", "2X");
+  }
+#undef GZ_UMMA_MX
+}
+
+// 32 rows x 16 bytes of shared memory -> four tensor-memory columns, repeated in the lanes of all four
+// warps: one tile of scales.  With a CTA pair each CTA's copy reads its own shared memory.
+template <int CTAS>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (CTAS == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// fp32 from the shared memory of another CTA of the cluster.
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
 // 32 lanes x 32 consecutive 32-bit columns of TMEM -> 32 registers per thread
 // (thread i of the warp reads lane base+i).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {

@@ -1,0 +1,311 @@
+"""Microscaled 4-bit matrices (include/gemmzoo/microscale.h): quantisation and its inverse, the
+product of two quantised matrices, and the gated feed-forward product.
+
+    q  = mx_quantize(x, MX_NVFP4)                          # rows x k, blocks along k
+    w  = mx_quantize(weight, MX_NVFP4, multiplier=256.0)   # n x k
+    MxGemm(m, n, k, MX_NVFP4, torch.bfloat16)(q, w, None, d, 1 / 256.0, 0.0)
+
+The reference (AD2605/gemm-zoo) has no counterpart: its narrowest type is 8 bits.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import api
+from .api import ACT_NONE, ACT_SILU, COL_MAJOR, GZ_OK, Epilogue, GzError, ROW_MAJOR, _ptr, _stream_handle, lib
+
+MX_FP4, MX_NVFP4 = 16, 17
+MX_CFG_AUTO, MX_CFG_PAIR, MX_CFG_SWAP_M16, MX_CFG_SWAP_M32, MX_CFG_SWAP_M64, MX_CFG_SWAP_M128 = 0, 1, 2, 3, 4, 5
+
+EXPORTED_SYMBOLS = [
+    "gz_mx_code_pitch", "gz_mx_scale_bytes", "gz_mx_quantize", "gz_mx_dequantize", "gz_mx_desc_validate",
+    "gz_mx_plan_create", "gz_mx_plan_destroy", "gz_mx_plan_info_get", "gz_mx_gemm_run", "gz_mx_gated_run",
+    "gz_mx_last_device_status",
+]
+
+
+class MxDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("format", C.c_int32), ("out_type", C.c_int32), ("gated", C.c_int32),
+        ("device", C.c_int32), ("config", C.c_int32), ("split", C.c_int32), ("flags", C.c_uint32),
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
+        ("pitch_a", C.c_int64), ("pitch_b", C.c_int64), ("ldc", C.c_int64), ("ldd", C.c_int64),
+        ("wait_limit_ns", C.c_uint64),
+    ]
+
+    @classmethod
+    def make(cls, format, out_type, m, n, k, gated=False, pitch_a=0, pitch_b=0, ldc=0, ldd=0, device=0,
+             config=MX_CFG_AUTO, split=0, flags=0, wait_limit_ns=0):
+        d = cls()
+        d.struct_size = C.sizeof(cls)
+        d.format, d.out_type, d.gated = format, out_type, int(gated)
+        d.device, d.config, d.split, d.flags = device, config, split, flags
+        d.m, d.n, d.k = m, n, k
+        d.pitch_a, d.pitch_b, d.ldc, d.ldd = pitch_a, pitch_b, ldc, ldd
+        d.wait_limit_ns = wait_limit_ns
+        return d
+
+
+class MxPlanInfo(C.Structure):
+    _fields_ = [
+        ("config", C.c_int32), ("split", C.c_int32), ("tile_m", C.c_int32), ("tile_n", C.c_int32),
+        ("tile_k", C.c_int32), ("stages", C.c_int32), ("grid", C.c_int32), ("smem_bytes", C.c_int32),
+        ("out_tma", C.c_int32), ("reserved", C.c_int32), ("tiles", C.c_int64),
+    ]
+
+    def as_dict(self):
+        return {f: getattr(self, f) for f, _ in self._fields_}
+
+
+_bound = None
+
+
+def _bind():
+    global _bound
+    if _bound is not None:
+        return _bound
+    L = lib()
+    vp, i32, i64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+    fp = C.POINTER(f32)
+    L.gz_mx_code_pitch.argtypes = [i64]
+    L.gz_mx_scale_bytes.argtypes = [i32, i64, i64]
+    L.gz_mx_quantize.argtypes = [vp, i32, i32, i64, i64, i64, i32, f32, vp, i64, vp, i32, vp]
+    L.gz_mx_dequantize.argtypes = [vp, i64, vp, i32, i64, i64, f32, vp, i32, i32, i64, i32, vp]
+    L.gz_mx_desc_validate.argtypes = [C.POINTER(MxDesc), C.c_int, C.POINTER(MxPlanInfo)]
+    L.gz_mx_plan_create.argtypes = [C.POINTER(vp), C.POINTER(MxDesc)]
+    L.gz_mx_plan_destroy.argtypes = [vp]
+    L.gz_mx_plan_info_get.argtypes = [vp, C.POINTER(MxPlanInfo)]
+    L.gz_mx_gemm_run.argtypes = [vp, vp, vp, vp, vp, vp, vp, fp, fp, C.POINTER(Epilogue), vp]
+    L.gz_mx_gated_run.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, fp, fp, i32, f32, vp]
+    L.gz_mx_last_device_status.argtypes = [vp, vp, C.POINTER(C.c_uint32 * 4)]
+    for name in EXPORTED_SYMBOLS:
+        getattr(L, name).restype = C.c_int
+    L.gz_mx_code_pitch.restype = i64
+    L.gz_mx_scale_bytes.restype = i64
+    _bound = L
+    return L
+
+
+def code_pitch(k: int) -> int:
+    """Bytes of one packed row of codes."""
+    return _bind().gz_mx_code_pitch(k)
+
+
+def scale_bytes(format: int, rows: int, k: int) -> int:
+    """Bytes of the scale array of a rows x k matrix."""
+    return _bind().gz_mx_scale_bytes(format, rows, k)
+
+
+class MxMatrix:
+    """A quantised rows x k matrix: `codes` (uint8, rows x pitch bytes) and `scales` (uint8, flat, in tiles of
+    128 rows x 4 blocks); the layout is that of include/gemmzoo/microscale.h."""
+
+    __slots__ = ("codes", "scales", "rows", "k", "format", "device", "pitch", "_codes_ptr", "_scales_ptr")
+
+    def __init__(self, codes, scales, rows, k, format):
+        import torch
+        need = scale_bytes(format, rows, k)
+        if need < 0:
+            raise ValueError("MxMatrix: rows and k must be positive and format one of MX_FP4, MX_NVFP4")
+        if not (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype == torch.uint8 and
+                scales.dtype == torch.uint8):
+            raise ValueError("MxMatrix: codes and scales are uint8 tensors")
+        if not (codes.is_cuda and codes.device == scales.device):
+            raise ValueError("MxMatrix: codes and scales must live on one CUDA device")
+        pitch = codes.stride(0) if codes.dim() == 2 and rows > 1 else codes.shape[-1]
+        if codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] < code_pitch(k) or codes.stride(1) != 1 or pitch % 16:
+            raise ValueError(f"MxMatrix: codes must be rows x at least {code_pitch(k)} bytes, contiguous along a row, "
+                             "rows a multiple of 16 bytes apart")
+        if not scales.is_contiguous() or scales.numel() < need:
+            raise ValueError(f"MxMatrix: scales must be {need} contiguous bytes")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise ValueError("MxMatrix: codes and scales must be 16-byte aligned")
+        self.codes, self.scales, self.rows, self.k, self.format = codes, scales, rows, k, format
+        self.device, self.pitch = codes.device.index, pitch
+        self._codes_ptr, self._scales_ptr = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def empty(cls, rows, k, format, device="cuda"):
+        """Uninitialised storage (the functions that write a quantised matrix write all of it)."""
+        import torch
+        need, pitch = scale_bytes(format, rows, k), code_pitch(k)
+        if need < 0:
+            raise ValueError("MxMatrix: rows and k must be positive and format one of MX_FP4, MX_NVFP4")
+        return cls(torch.empty(rows, pitch, dtype=torch.uint8, device=device),
+                   torch.empty(need, dtype=torch.uint8, device=device), rows, k, format)
+
+
+def tile_scales(linear, format):
+    """rows x blocks scale bytes (one row after the other, as checkpoints hold them) -> the tiled array."""
+    import torch
+    rows, blocks = linear.shape
+    rg, bg = -(-rows // 128), -(-blocks // 4)
+    s = torch.zeros(rg * 128, bg * 4, dtype=torch.uint8, device=linear.device)
+    s[:rows, :blocks] = linear.view(torch.uint8)
+    return s.view(rg, 4, 32, bg, 4).permute(0, 3, 2, 1, 4).reshape(-1)
+
+
+def linear_scales(q: MxMatrix):
+    """The inverse of tile_scales: the rows x blocks scale bytes of a quantised matrix."""
+    blocks = -(-q.k // (16 if q.format == MX_NVFP4 else 32))
+    rg, bg = -(-q.rows // 128), -(-blocks // 4)
+    s = q.scales[:rg * bg * 512].view(rg, bg, 32, 4, 4).permute(0, 3, 2, 1, 4)
+    return s.reshape(rg * 128, bg * 4)[:q.rows, :blocks].contiguous()
+
+
+def _matrix_args(x, layout, what):
+    """rows, k, ld of a 2-D tensor in `layout` (row-major: rows x k; column-major: k x rows)."""
+    if x.dim() != 2 or not x.is_cuda:
+        raise ValueError(f"{what}: a 2-D CUDA tensor is needed")
+    d0, d1 = x.shape
+    if d1 > 1 and x.stride(1) != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    ld = x.stride(0) if d0 > 1 else d1
+    if ld < d1:
+        raise ValueError(f"{what}: rows overlap")
+    return (d0, d1, ld) if layout == ROW_MAJOR else (d1, d0, ld)
+
+
+def mx_quantize(x, format, layout=ROW_MAJOR, multiplier=1.0, out=None, stream=None):
+    """Quantise x * multiplier along k (gz_mx_quantize).  x: 2-D, rows x k (ROW_MAJOR) or k x rows (COL_MAJOR).
+    Returns `out`, or a new MxMatrix."""
+    rows, k, ld = _matrix_args(x, layout, "mx_quantize")
+    if out is None:
+        if stream is None or isinstance(stream, int):
+            out = MxMatrix.empty(rows, k, format, x.device)
+        else:
+            import torch
+            with torch.cuda.stream(stream):  # the allocator then knows the memory's stream
+                out = MxMatrix.empty(rows, k, format, x.device)
+    elif out.rows != rows or out.k != k or out.format != format or out.device != x.device.index:
+        raise ValueError("mx_quantize: out has another size, format or device")
+    st = _bind().gz_mx_quantize(x.data_ptr(), api._torch_dtype_code(x.dtype), layout, ld, rows, k, format, multiplier,
+                                out._codes_ptr, out.pitch, out._scales_ptr, out.device, _stream_handle(stream))
+    if st != GZ_OK:
+        raise GzError(st, "gz_mx_quantize")
+    return out
+
+
+def mx_dequantize(q: MxMatrix, out, layout=ROW_MAJOR, multiplier=1.0, stream=None):
+    """code * scale * multiplier into `out` (gz_mx_dequantize), a 2-D tensor in `layout`.  Returns `out`."""
+    rows, k, ld = _matrix_args(out, layout, "mx_dequantize")
+    if q.rows != rows or q.k != k or q.device != out.device.index:
+        raise ValueError("mx_dequantize: out has another size or device")
+    st = _bind().gz_mx_dequantize(q._codes_ptr, q.pitch, q._scales_ptr, q.format, rows, k, multiplier, out.data_ptr(),
+                                  api._torch_dtype_code(out.dtype), layout, ld, q.device, _stream_handle(stream))
+    if st != GZ_OK:
+        raise GzError(st, "gz_mx_dequantize")
+    return out
+
+
+def mx_validate(desc: MxDesc, sm_count: int = 0):
+    """Host-only validation.  Returns (status, MxPlanInfo)."""
+    info = MxPlanInfo()
+    st = _bind().gz_mx_desc_validate(C.byref(desc), sm_count, C.byref(info))
+    return st, info
+
+
+class _MxPlan:
+    """Owns a gz_mx_plan."""
+
+    def __init__(self, desc: MxDesc):
+        self.desc = desc
+        self._h = C.c_void_p()
+        h = C.c_void_p()
+        st = _bind().gz_mx_plan_create(C.byref(h), C.byref(desc))
+        if st != GZ_OK:
+            raise GzError(st, "gz_mx_plan_create")
+        self._h = h
+
+    def info(self) -> MxPlanInfo:
+        info = MxPlanInfo()
+        st = _bind().gz_mx_plan_info_get(self._h, C.byref(info))
+        if st != GZ_OK:
+            raise GzError(st, "gz_mx_plan_info_get")
+        return info
+
+    def device_status(self, stream=None):
+        """(status, detail[4]) after synchronising `stream`."""
+        detail = (C.c_uint32 * 4)()
+        st = _bind().gz_mx_last_device_status(self._h, _stream_handle(stream), C.byref(detail))
+        return st, list(detail)
+
+    def destroy(self):
+        if self._h:
+            _bind().gz_mx_plan_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+    def _check(self, name, q, rows, k, pitch):
+        if q.rows != rows or q.k != k or q.format != self.desc.format or q.device != self.desc.device or q.pitch != pitch:
+            raise ValueError(f"{name}: expected {rows} x {k}, format {self.desc.format}, pitch {pitch} on device {self.desc.device}, "
+                             f"got {q.rows} x {q.k}, format {q.format}, pitch {q.pitch} on device {q.device}")
+
+
+def _out_code(t):
+    return t if isinstance(t, int) else api._torch_dtype_code(t)
+
+
+class MxGemm(_MxPlan):
+    """D[m x n] = act(alpha * row_scale * col_scale * A B^T + beta * C + bias) for quantised A (m x k) and
+    B (n x k) (gz_mx_gemm_run).  pitch_a / pitch_b: bytes between rows of codes, 0 = packed."""
+
+    def __init__(self, m, n, k, format, out_dtype, ldc=0, ldd=0, pitch_a=0, pitch_b=0, device=0, config=MX_CFG_AUTO,
+                 split=0, flags=0, wait_limit_ns=0):
+        super().__init__(MxDesc.make(format, _out_code(out_dtype), m, n, k, False, pitch_a, pitch_b, ldc, ldd, device,
+                                     config, split, flags, wait_limit_ns))
+        self._m, self._n, self._k = m, n, k
+        self._pa, self._pb = pitch_a or code_pitch(k), pitch_b or code_pitch(k)
+
+    def __call__(self, a: MxMatrix, b: MxMatrix, c, d, alpha, beta, bias=None, row_scale=None, col_scale=None,
+                 activation=ACT_NONE, stream=None):
+        self._check("a", a, self._m, self._k, self._pa)
+        self._check("b", b, self._n, self._k, self._pb)
+        ep = None
+        if bias is not None or row_scale is not None or col_scale is not None or activation != ACT_NONE:
+            ep = C.byref(Epilogue.make(bias, row_scale, col_scale, activation))
+        st = _bind().gz_mx_gemm_run(self._h, a._codes_ptr, a._scales_ptr, b._codes_ptr, b._scales_ptr, _ptr(c), _ptr(d),
+                                    C.byref(C.c_float(alpha)), C.byref(C.c_float(beta)), ep, _stream_handle(stream))
+        if st != GZ_OK:
+            raise GzError(st, "gz_mx_gemm_run")
+
+
+class MxGated(_MxPlan):
+    """D[m x n] = act(alpha_gate * A G^T) * (alpha_up * A U^T) for quantised A (m x k), gate and up (n x k) in one
+    launch (gz_mx_gated_run).  out_dtype: a torch type (or DT_* code) for a plain D, or MX_FP4 / MX_NVFP4 for an
+    MxMatrix, which then holds D * out_multiplier."""
+
+    def __init__(self, m, n, k, format, out_dtype, activation=ACT_SILU, ldd=0, pitch_a=0, pitch_b=0, device=0,
+                 config=MX_CFG_AUTO, split=0, flags=0, wait_limit_ns=0):
+        super().__init__(MxDesc.make(format, _out_code(out_dtype), m, n, k, True, pitch_a, pitch_b, 0, ldd, device,
+                                     config, split, flags, wait_limit_ns))
+        self.activation = activation
+        self._m, self._n, self._k = m, n, k
+        self._pa, self._pb = pitch_a or code_pitch(k), pitch_b or code_pitch(k)
+        self._out = self.desc.out_type
+        self._quantised = self._out in (MX_FP4, MX_NVFP4)
+        self._pd = ldd or (code_pitch(n) if self._quantised else 0)
+
+    def __call__(self, a: MxMatrix, gate: MxMatrix, up: MxMatrix, d, alpha_gate=1.0, alpha_up=1.0, out_multiplier=1.0,
+                 stream=None):
+        self._check("a", a, self._m, self._k, self._pa)
+        self._check("gate", gate, self._n, self._k, self._pb)
+        self._check("up", up, self._n, self._k, self._pb)
+        if self._quantised:
+            if not isinstance(d, MxMatrix) or (d.rows, d.k, d.format, d.device, d.pitch) != (
+                    self._m, self._n, self._out, self.desc.device, self._pd):
+                raise ValueError("d: an MxMatrix of the output's size, format, pitch and device is needed")
+            dp, ds = d._codes_ptr, d._scales_ptr
+        else:
+            dp, ds = _ptr(d), None
+        st = _bind().gz_mx_gated_run(self._h, a._codes_ptr, a._scales_ptr, gate._codes_ptr, gate._scales_ptr,
+                                     up._codes_ptr, up._scales_ptr, dp, ds, C.byref(C.c_float(alpha_gate)),
+                                     C.byref(C.c_float(alpha_up)), self.activation, out_multiplier,
+                                     _stream_handle(stream))
+        if st != GZ_OK:
+            raise GzError(st, "gz_mx_gated_run")
