@@ -18,7 +18,7 @@ from .api import (  # noqa: F401
     ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU, Epilogue,
 )
 from .microscale import (  # noqa: F401
-    MX_FP4, MX_NVFP4, MX_CFG_AUTO, MX_CFG_PAIR, MX_CFG_SWAP_M16, MX_CFG_SWAP_M32, MX_CFG_SWAP_M64, MX_CFG_SWAP_M128,
+    MX_FP4, MX_NVFP4, MX_CFG_AUTO, MX_CFG_PAIR, MX_CFG_SINGLE, MX_CFG_SWAP_M16, MX_CFG_SWAP_M32, MX_CFG_SWAP_M64,
     MxDesc, MxGated, MxGemm, MxMatrix, MxPlanInfo, linear_scales, mx_dequantize, mx_quantize, mx_validate, tile_scales,
 )
 

@@ -57,20 +57,21 @@ gz_status mx_quant_params(gz::mx::QuantParams* p, const void* values, int type, 
   p->code_bytes = gz_mx_code_pitch(k);
   p->groups = mx_groups(format, k);
   p->multiplier = multiplier;
+  p->unit = multiplier == 1.0f ? 1u : 0u;
   const uintptr_t vec = cols ? 16 : 32;  // bytes per access of the two kernels
   p->vec = (mx_aligned(values, vec) && (ld * size) % (int64_t)vec == 0) ? 1u : 0u;
   return GZ_OK;
 }
 
 struct MxShape {
-  int config, bn;
-  bool pair;
+  int config, bn, ctas;
+  bool swap() const { return bn < 256; }
 };
-const MxShape kMxShapes[] = {{GZ_MX_CFG_PAIR, 256, true},
-                             {GZ_MX_CFG_SWAP_M16, 16, false},
-                             {GZ_MX_CFG_SWAP_M32, 32, false},
-                             {GZ_MX_CFG_SWAP_M64, 64, false},
-                             {GZ_MX_CFG_SWAP_M128, 128, false}};
+const MxShape kMxShapes[] = {{GZ_MX_CFG_PAIR, 256, 2},
+                             {GZ_MX_CFG_SINGLE, 256, 1},
+                             {GZ_MX_CFG_SWAP_M16, 16, 1},
+                             {GZ_MX_CFG_SWAP_M32, 32, 1},
+                             {GZ_MX_CFG_SWAP_M64, 64, 1}};
 const MxShape* mx_shape_of(int config) {
   for (const auto& s : kMxShapes)
     if (s.config == config) return &s;
@@ -113,43 +114,75 @@ gz_status mx_normalise(const gz_mx_desc* desc, MxProblem* pr) {
   return GZ_OK;
 }
 
-bool mx_shape_fits(const MxProblem& pr, const MxShape& s) { return s.pair || s.bn == 128 || pr.d.m <= s.bn; }
+bool mx_shape_fits(const MxProblem& pr, const MxShape& s) { return !s.swap() || pr.d.m <= s.bn; }
 
 int64_t mx_tiles(const MxProblem& pr, const MxShape& s) {
-  if (s.pair) return cdiv(pr.d.m, 256) * cdiv(pr.d.n, pr.d.gated ? 128 : 256);
-  return cdiv(pr.d.n, 128) * cdiv(pr.d.m, s.bn);
+  if (!s.swap()) return cdiv(pr.d.m, 128 * s.ctas) * cdiv(pr.d.n, pr.d.gated ? 128 : 256);
+  return cdiv(pr.d.n, 128);
 }
 
-// CTAs that share a tile's K range: as many as keep every tile in one wave, with at least two K blocks
-// each (a CTA's set-up and the meeting of the partial sums cost about as much as two).
-int mx_split(const MxProblem& pr, const MxShape& s, int sm_count) {
-  if (s.pair) return 1;
+// The largest cluster is eight CTAs, and a row tile has four (gated) or eight slices of 32 columns to
+// deal to the parts.
+int mx_max_split(const MxProblem& pr, const MxShape& s) { return (s.ctas == 2 || (!s.swap() && pr.d.gated)) ? 4 : 8; }
+
+// CTAs that can be resident at the same time in clusters of `cluster`.  A cluster lies within one GPC;
+// 148 SMs in GPCs of 16 to 20 hold 16 clusters of eight or 33 of four one-per-SM CTAs.  Swapped tiles have
+// two CTAs per SM.
+int64_t mx_resident(const MxShape& s, int cluster, int sm_count) {
+  const int64_t sms = cluster >= 8 ? sm_count * 128 / 148 : cluster == 4 ? sm_count * 132 / 148 : sm_count;
+  return s.swap() ? 2 * sms : sms;
+}
+
+// Clocks that a configuration is estimated to take; see DESIGN for what the constants were fitted to.
+double mx_cost(const MxProblem& pr, const MxShape& s, int split, int sm_count) {
   const int64_t tiles = mx_tiles(pr, s), k_blocks = cdiv(pr.d.k, 256);
-  // clusters of eight leave SMs over in each GPC: 16 of them fit
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sm_count - (split == 4 ? 20 : split == 2 ? 16 : 0) && k_blocks >= 4 * split) split *= 2;
-  return split;
+  const bool nv = pr.d.format == GZ_MX_NVFP4;
+  const double mb = (s.swap() && pr.d.gated) ? 2.0 : 1.0;
+  const double bytes = (128.0 * mb + double(s.bn) / s.ctas) * 128.0 + 512.0 * (nv ? 4 : 2) * (mb + (s.swap() ? 1 : 2));
+  const int64_t slots = mx_resident(s, s.ctas * split, sm_count) / (s.ctas * split);  // clusters
+  if (slots <= 0) return 1e30;
+  const double waves = double(cdiv(tiles, slots));
+  const double blocks = double(cdiv(k_blocks, split));
+  // clocks per K block: the MMAs; the fill from L2 (and, for all CTAs together, from HBM)
+  const double mma = s.swap() ? 200.0 * mb : 512.0;
+  const double active = double(tiles * s.ctas * split < slots * s.ctas * split ? tiles * s.ctas * split : slots * s.ctas * split);
+  const double per_sm = s.swap() && active > sm_count ? 2.0 : 1.0;
+  double per_block = bytes / 60.0 * per_sm;
+  if (mma > per_block) per_block = mma;
+  if (s.swap() && bytes * active / 3400.0 > per_block) per_block = bytes * active / 3400.0;
+  const double finish = s.swap() ? 600.0 + 12.0 * double(pr.d.m) * mb / split : 3000.0 + (split > 1 ? 2500.0 : 0.0);
+  const double fixed = 4000.0 + (s.ctas == 2 ? 1500.0 : 0.0) + (split > 1 ? 1500.0 : 0.0);
+  if (s.swap()) return waves * (blocks * per_block + finish) + fixed;
+  return waves * (blocks * per_block + 300.0) + finish + fixed;
+}
+
+int mx_choose_split(const MxProblem& pr, const MxShape& s, int sm_count, double* cost) {
+  const int64_t tiles = mx_tiles(pr, s), k_blocks = cdiv(pr.d.k, 256);
+  int best = 1;
+  *cost = mx_cost(pr, s, 1, sm_count);
+  for (int split = 2; split <= mx_max_split(pr, s); split *= 2) {
+    if (k_blocks < split || tiles * s.ctas * split > mx_resident(s, s.ctas * split, sm_count)) break;
+    const double c = mx_cost(pr, s, split, sm_count);
+    if (c < *cost) {
+      *cost = c;
+      best = split;
+    }
+  }
+  return best;
 }
 
 int mx_choose(const MxProblem& pr, int sm_count) {
   double best = 0;
-  int best_cfg = GZ_MX_CFG_SWAP_M128;
-  const double k_blocks = double(cdiv(pr.d.k, 256));
+  int best_cfg = GZ_MX_CFG_SINGLE;
   for (const auto& s : kMxShapes) {
-    if (!mx_shape_fits(pr, s)) continue;
-    const int64_t units = s.pair ? sm_count / 2 : sm_count;
-    if (units <= 0) continue;
-    const int64_t tiles = mx_tiles(pr, s);
-    const int split = pr.d.split ? pr.d.split : mx_split(pr, s, sm_count);
-    const double mb = s.pair ? 1.0 : pr.d.gated ? 2.0 : 1.0;
-    const double rows = s.pair ? 128.0 : double(s.bn);  // of the narrow side that a CTA loads
-    const double mma = s.pair ? 512.0 : 4.0 * mb * (s.bn / 2.0 > 32.0 + s.bn / 4.0 ? s.bn / 2.0 : 32.0 + s.bn / 4.0);
-    const double bytes = (128.0 * mb + rows) * 128.0 + 512.0 * (pr.d.format == GZ_MX_NVFP4 ? 4 : 2) * (mb + (s.pair ? 2 : 1));
-    double per_block = mma > bytes / 48.0 ? mma : bytes / 48.0;
-    if (per_block < 250.0) per_block = 250.0;
-    const double waves = double(cdiv(tiles * split, units));
-    const double fixed = (s.pair ? 6000.0 : 3000.0) + 8.0 * s.bn * mb;
-    const double cost = waves * (k_blocks / split * per_block + 500.0) + fixed + (split > 1 ? 1500.0 : 0.0);
+    if (!mx_shape_fits(pr, s) || sm_count < s.ctas) continue;
+    double cost;
+    if (pr.d.split) {
+      if (pr.d.split > mx_max_split(pr, s)) continue;
+      cost = mx_cost(pr, s, pr.d.split, sm_count);
+    } else {
+      mx_choose_split(pr, s, sm_count, &cost);
+    }
     if (best == 0 || cost < best) {
       best = cost;
       best_cfg = s.config;
@@ -168,23 +201,25 @@ gz_status mx_resolve(const MxProblem& pr, int sm_count, gz_mx_plan_info* info) {
   const MxShape& s = *mx_shape_of(config);
   if (!mx_shape_fits(pr, s)) return GZ_ERR_UNSUPPORTED;
   const int64_t tiles = mx_tiles(pr, s);
-  int split = pr.d.split ? pr.d.split : mx_split(pr, s, sm_count);
-  if (s.pair && split != 1) return GZ_ERR_UNSUPPORTED;
-  // a shared K range is one wave of clusters, each CTA with a part of it
-  if (split > 1 && (tiles * split > sm_count || cdiv(pr.d.k, 256) < split)) return GZ_ERR_UNSUPPORTED;
+  double cost;
+  const int split = pr.d.split ? pr.d.split : mx_choose_split(pr, s, sm_count, &cost);
+  if (split > mx_max_split(pr, s) || sm_count < s.ctas) return GZ_ERR_UNSUPPORTED;
+  // a shared K range: every CTA has a part of it, and a row tile's cluster has one tile
+  if (split > 1 && cdiv(pr.d.k, 256) < split) return GZ_ERR_UNSUPPORTED;
   const gz::MxEntry e = mx_entry_of(pr, config);
   std::memset(info, 0, sizeof(*info));
   info->config = config;
   info->split = split;
-  info->tile_m = s.pair ? 256 : s.bn;
-  info->tile_n = s.pair ? (pr.d.gated ? 128 : 256) : 128;
+  info->tile_m = s.swap() ? s.bn : 128 * s.ctas;
+  info->tile_n = s.swap() || pr.d.gated ? 128 : 256;
   info->tile_k = 256;
   info->stages = e.stages;
   info->smem_bytes = e.smem_bytes;
-  const int64_t units = s.pair ? sm_count / 2 : split > 1 ? tiles : sm_count;
-  if (units <= 0) return GZ_ERR_UNSUPPORTED;
-  info->grid = (int32_t)((tiles < units ? tiles : units) * (s.pair ? 2 : split));
-  info->out_tma = (s.pair && pr.out_size != 0 && (pr.d.ldd * pr.out_size) % 16 == 0 &&
+  const int64_t walkers = sm_count / s.ctas;  // CTAs or pairs that walk the tiles of a persistent launch
+  const int64_t clusters = s.swap() || split > 1 || tiles < walkers ? tiles : walkers;
+  if (clusters * s.ctas * split > (int64_t(1) << 31) - 1) return GZ_ERR_TOO_LARGE;
+  info->grid = (int32_t)(clusters * s.ctas * split);
+  info->out_tma = (!s.swap() && pr.out_size != 0 && (pr.d.ldd * pr.out_size) % 16 == 0 &&
                    pr.d.ldd * pr.out_size < (int64_t(1) << 40)) ? 1 : 0;
   info->tiles = tiles;
   return GZ_OK;
@@ -244,7 +279,7 @@ gz_status mx_launch(gz_mx_plan* pl, gz::MxParams* p, const void* a, const void* 
   const MxShape& s = *mx_shape_of(pl->info.config);
   gz::MxMaps maps;
   bool ok;
-  if (s.pair)
+  if (!s.swap())
     ok = mx_encode_operand(pl, &maps.wide, &maps.wide_scales, a, a_scales, d.m, d.pitch_a, 128) &&
          mx_encode_operand(pl, &maps.narrow, &maps.narrow_scales, b, b_scales, d.n, d.pitch_b, 128);
   else
@@ -256,6 +291,9 @@ gz_status mx_launch(gz_mx_plan* pl, gz::MxParams* p, const void* a, const void* 
     maps.up = maps.narrow;
     maps.up_scales = maps.narrow_scales;
   }
+  // four columns at a time in the swapped tiles' epilogue
+  const int64_t quad = 4 * pl->pr.out_size;
+  p->d_vec_ok = (quad != 0 && mx_aligned(p->d, quad) && d.ldd % 4 == 0 && (!p->c || (mx_aligned(p->c, quad) && d.ldc % 4 == 0))) ? 1u : 0u;
   p->out_tma = (pl->info.out_tma && mx_aligned(p->d, 16)) ? 1u : 0u;
   if (p->out_tma) {
     const bool f32 = d.out_type == GZ_DT_F32;
@@ -266,7 +304,7 @@ gz_status mx_launch(gz_mx_plan* pl, gz::MxParams* p, const void* a, const void* 
   } else {
     maps.d = maps.wide;  // unused by the kernel
   }
-  if (!cuda_ok(pl->entry.launch(maps, *p, pl->info.grid, s.pair ? 2 : pl->info.split, stream), "kernel launch"))
+  if (!cuda_ok(pl->entry.launch(maps, *p, pl->info.grid, s.ctas * pl->info.split, stream), "kernel launch"))
     return GZ_ERR_CUDA;
   return GZ_OK;
 }
@@ -289,24 +327,12 @@ GZ_API gz_status gz_mx_quantize(const void* src, int32_t src_type, int32_t layou
   gz_status st = mx_quant_params(&p, src, src_type, layout, ld, rows, k, format, multiplier, codes, pitch, scales, device);
   if (st != GZ_OK) return st;
   const bool nv = format == GZ_MX_NVFP4, cols = layout == GZ_COL_MAJOR;
-  int64_t blocks;
-  if (cols) {
-    blocks = cdiv(rows, 128) * 2 * cdiv(k, 128);
-  } else {
-    const int64_t word = nv ? 4 : 8;  // 16-element chunks per word of scales
-    const int64_t per_row = cdiv(cdiv(k, 16), word) * word;
-    p.per_row = (uint32_t)per_row;
-    p.items = cdiv(rows, 128) * 128 * per_row;
-    blocks = cdiv(p.items, 256);
-  }
-  if (blocks > kMxExtent) return GZ_ERR_TOO_LARGE;
-  if ((st = mx_device_ok(device)) != GZ_OK) return st;
   DeviceGuard guard(device);
-  if (!guard.ok()) return GZ_ERR_CUDA;
+  if (!guard.ok()) return (st = mx_device_ok(device)) != GZ_OK ? st : GZ_ERR_CUDA;
   p.in = src;
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
-  if (!cuda_ok(gz::mx_launch_quantize(src_type, nv, cols, p, blocks, static_cast<cudaStream_t>(stream)), "kernel launch"))
+  if (!cuda_ok(gz::mx_launch_quantize(src_type, nv, cols, p, static_cast<cudaStream_t>(stream)), "kernel launch"))
     return GZ_ERR_CUDA;
   return GZ_OK;
 }
@@ -318,22 +344,12 @@ GZ_API gz_status gz_mx_dequantize(const void* codes, int64_t pitch, const void* 
   gz_status st = mx_quant_params(&p, dst, dst_type, layout, ld, rows, k, format, multiplier, codes, pitch, scales, device);
   if (st != GZ_OK) return st;
   const bool nv = format == GZ_MX_NVFP4, cols = layout == GZ_COL_MAJOR;
-  int64_t blocks;
-  if (cols) {
-    blocks = cdiv(rows, gz::mx::COL_ROWS) * cdiv(k, gz::mx::COL_K);
-  } else {
-    p.per_row = (uint32_t)cdiv(k, 16);
-    p.items = rows * (int64_t)p.per_row;
-    blocks = cdiv(p.items, 256);
-  }
-  if (blocks > kMxExtent) return GZ_ERR_TOO_LARGE;
-  if ((st = mx_device_ok(device)) != GZ_OK) return st;
   DeviceGuard guard(device);
-  if (!guard.ok()) return GZ_ERR_CUDA;
+  if (!guard.ok()) return (st = mx_device_ok(device)) != GZ_OK ? st : GZ_ERR_CUDA;
   p.out = dst;
   p.codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
   p.scales = const_cast<uint8_t*>(static_cast<const uint8_t*>(scales));
-  if (!cuda_ok(gz::mx_launch_dequantize(dst_type, nv, cols, p, blocks, static_cast<cudaStream_t>(stream)), "kernel launch"))
+  if (!cuda_ok(gz::mx_launch_dequantize(dst_type, nv, cols, p, static_cast<cudaStream_t>(stream)), "kernel launch"))
     return GZ_ERR_CUDA;
   return GZ_OK;
 }
@@ -381,9 +397,9 @@ GZ_API gz_status gz_mx_plan_create(gz_mx_plan** out, const gz_mx_desc* desc) {
   const MxShape& s = *mx_shape_of(info.config);
   gz::MxParams& p = pl->base;
   std::memset(&p, 0, sizeof(p));
-  p.grid.tiles_m = (uint32_t)(s.pair ? cdiv(d.m, 256) : cdiv(d.n, 128));
-  p.grid.tiles_n = (uint32_t)(s.pair ? cdiv(d.n, info.tile_n) : cdiv(d.m, s.bn));
-  p.grid.group_m = s.pair ? 8u : 16u;  // about 2048 rows of output per group, as for the 8- and 16-bit tiles
+  p.grid.tiles_m = (uint32_t)(s.swap() ? cdiv(d.n, 128) : cdiv(d.m, 128 * s.ctas));
+  p.grid.tiles_n = (uint32_t)(s.swap() ? 1 : cdiv(d.n, info.tile_n));
+  p.grid.group_m = s.ctas == 2 ? 8u : 16u;  // about 2048 rows of output per group, as for the 8- and 16-bit tiles
   p.grid.num_tiles = p.grid.tiles_m * p.grid.tiles_n;
   p.m = (uint32_t)d.m;
   p.n = (uint32_t)d.n;
@@ -391,7 +407,7 @@ GZ_API gz_status gz_mx_plan_create(gz_mx_plan** out, const gz_mx_desc* desc) {
   p.split = (uint32_t)info.split;
   // e2m1 operands, N, scale type, M
   p.idesc = (1u << 7) | (1u << 10) | ((uint32_t)(s.bn >> 3) << 17) | ((d.format == GZ_MX_FP4 ? 1u : 0u) << 23) |
-            ((s.pair ? 256u >> 4 : 128u >> 4) << 24);
+            ((uint32_t)(8 * s.ctas) << 24);
   p.out_type = (uint32_t)d.out_type;
   p.test_flags = (d.flags & GZ_FLAG_TEST_WITHHOLD_ACC_READY) ? 1u : 0u;
   p.ldc = d.ldc;

@@ -69,12 +69,13 @@ __device__ __forceinline__ Scale block_scale(float amax) {
 // residual correction of x * (1/s) (Markstein's theorem: with a correctly rounded reciprocal the
 // corrected quotient is correctly rounded).  Correct rounding suffices: the rounding borders of e2m1
 // have 3 significant bits and the scale 4, so border * scale is an fp32 number and an x beside it
-// differs from it by at least one unit of x, which is more than half a unit of the quotient.
+// differs from it by at least one unit of x, which is more than half a unit of the quotient.  The
+// residual is taken as q s - x, so that an exact quotient, -0 among them, comes through unchanged.
 template <bool NV>
 __device__ __forceinline__ float in_code_units(float x, const Scale& s) {
   if constexpr (!NV) return x * s.inv;
   const float q = x * s.inv;
-  return copysignf(fmaf(fmaf(-q, s.value, x), s.inv, q), x);  // the correction would make +0 of -0
+  return fmaf(-fmaf(q, s.value, -x), s.inv, q);
 }
 
 // Eight values in code units -> eight e2m1 codes, the first in the low nibble (ties to even,

@@ -12,19 +12,24 @@
 // in tensor memory need no barrier of their own.
 //
 // Two tile families:
-//   pair     256 x 256 on a CTA pair (cta_group::2): A's rows on the 128-lane side, each CTA with its
-//            own 128 rows of A and its own 128 rows of B; scales of all 256 rows of B in both.  The
-//            gated product gives CTA 0 the gate's 128 rows and CTA 1 the up projection's: one MMA
-//            computes both halves and no operand is loaded twice.  Two fp32 accumulators of 256
-//            columns would fill tensor memory and leave no room for scales, so they overlap in 64
-//            columns: [0, 256) and [192, 448).  The epilogue reads the shared 64 columns first and
-//            the next tile's main loop starts while it works on the other 192.
-//   swapped  few rows of A: B's rows on the 128-lane side (128 features per tile), 16 to 128 rows of A
-//            on the narrow side, so every byte a stage loads is a useful byte of B.  The gated product
-//            keeps two row blocks per stage (gate and up).  Where tiles are fewer than SMs, a cluster
-//            of up to eight CTAs shares a tile's K range; the partial sums meet in shared memory
-//            (each CTA adds a share of the rows over distributed shared memory, in rank order), so there
-//            is no workspace, nothing to clear and one order of summation.
+//   row tiles  256 x 256 on a CTA pair (cta_group::2) or 128 x 256 on one CTA: A's rows on the 128-lane
+//              side.  In a pair each CTA loads its own 128 rows of A and its own 128 rows of B, and the
+//              scales of all 256 rows of B.  The gated product takes 128 rows of the gate and 128 of the
+//              up projection as its 256 (in a pair CTA 0 loads the gate's, CTA 1 the up projection's):
+//              one MMA computes both halves and no operand is loaded twice.  Two fp32 accumulators of
+//              256 columns would fill tensor memory and leave no room for scales, so they overlap in 64
+//              columns: [0, 256) and [192, 448).  The epilogue reads the shared 64 columns first and
+//              the next tile's main loop starts while it works on the other 192.
+//   swapped    few rows of A: B's rows on the 128-lane side (128 features per tile), 16, 32 or 64 rows of
+//              A on the narrow side, so every byte a stage loads is a useful byte of B.  The gated
+//              product keeps two row blocks per stage (gate and up).  One tile per CTA and shared memory
+//              for two CTAs per SM: one streams while the other starts or finishes.  The accumulator
+//              is the transpose of the output; it goes through shared memory, after which a warp takes
+//              one output row at a time, a lane four neighbouring columns.
+// Where tiles are fewer than SMs, the CTAs (pairs) of a cluster share a tile's K range.  Their partial
+// sums meet in shared memory, in the ring that the main loop no longer needs; each CTA adds and
+// finishes a share of the tile over distributed shared memory, in rank order, so there is no
+// workspace, nothing to clear and one order of summation.
 #ifndef GZ_MX_GEMM_CUH
 #define GZ_MX_GEMM_CUH
 
@@ -39,7 +44,7 @@ constexpr uint32_t MX_OUT_FP4 = 16, MX_OUT_NVFP4 = 17;
 struct MxMaps {
   CUtensorMap wide, wide_scales;      // the operand on the 128-lane side
   CUtensorMap narrow, narrow_scales;  // the other one
-  CUtensorMap up, up_scales;          // gated: the up projection (the gate is `wide` of a swapped tile, `narrow` of a pair)
+  CUtensorMap up, up_scales;          // gated: the up projection (the gate is `wide` of a swapped tile, `narrow` of a row tile)
   CUtensorMap d;
 };
 
@@ -47,10 +52,11 @@ struct MxParams {
   TileGrid grid;  // tiles_m along the 128-lane side
   uint32_t m, n;  // rows and columns of the output
   uint32_t k_blocks;
-  uint32_t split;  // swapped tiles: CTAs (one cluster) that share a tile's K range
+  uint32_t split;  // CTAs or CTA pairs (one cluster) that share a tile's K range
   uint32_t idesc;
   uint32_t out_type;
   uint32_t out_tma, c_vec_ok;
+  uint32_t d_vec_ok;  // swapped tiles: four columns of C and of D may be accessed at once
   uint32_t test_flags;
   uint32_t epi_flags, act;  // bit 0 bias, 1 row_scale, 2 col_scale
   float alpha, alpha_up, beta, out_multiplier;
@@ -66,37 +72,38 @@ struct MxParams {
   uint64_t wait_limit_ns;
 };
 
-template <bool NV_, int BN_, bool PAIR_, bool GATED_>
+template <bool NV_, int BN_, int CTAS_, bool GATED_>
 struct MxCfg {
-  static constexpr bool NV = NV_, PAIR = PAIR_, GATED = GATED_;
-  static constexpr int BN = BN_;
-  static constexpr int CTAS = PAIR ? 2 : 1;
-  static constexpr int MB = (GATED && !PAIR) ? 2 : 1;  // 128-row blocks on the wide side per CTA
-  static constexpr int TILES_K = NV ? 4 : 2;           // scale tiles per stage and 128 rows
-  static constexpr int NRB = BN > 128 ? 2 : 1;         // scale row groups of the narrow side
+  static constexpr bool NV = NV_, GATED = GATED_;
+  static constexpr int BN = BN_, CTAS = CTAS_;
+  static constexpr bool SWAP = BN < 256;
+  static constexpr int MB = (GATED && SWAP) ? 2 : 1;  // 128-row blocks on the wide side per CTA
+  static constexpr int TILES_K = NV ? 4 : 2;          // scale tiles per stage and 128 rows
+  static constexpr int NRB = SWAP ? 1 : 2;            // scale row groups of the narrow side
   static constexpr int W_BYTES = MB * 128 * 128;
   static constexpr int N_BYTES = (BN / CTAS) * 128;
   static constexpr int WS_BYTES = MB * TILES_K * 512;
   static constexpr int NS_BYTES = NRB * TILES_K * 512;
   static constexpr int STAGE_BYTES = W_BYTES + N_BYTES + WS_BYTES + NS_BYTES;
-  static constexpr int EPI_WARPS = PAIR ? 8 : 4;
-  static constexpr int STAGING_BYTES = PAIR ? EPI_WARPS * 4096 : 0;
+  static constexpr int EPI_WARPS = SWAP ? 4 : 8;
+  static constexpr int STAGING_BYTES = SWAP ? 0 : EPI_WARPS * 4096;
   static constexpr int BAR_BYTES = 512;
-  static constexpr int MAX_STAGES = (232448 - 1024 - STAGING_BYTES - BAR_BYTES) / STAGE_BYTES;
-  static constexpr int STAGES = MAX_STAGES < 12 ? MAX_STAGES : 12;
+  // 227 KB per block; two blocks per SM share 228 KB of which each costs 1 KB more than it asks for
+  static constexpr int SMEM_LIMIT = SWAP ? 115712 : 232448;
+  static constexpr int STAGES = (SMEM_LIMIT - 1024 - STAGING_BYTES - BAR_BYTES) / STAGE_BYTES;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int SMEM_BYTES = 1024 + RING_BYTES + STAGING_BYTES + BAR_BYTES;
   static constexpr int THREADS = 96 + 32 * EPI_WARPS;
-  // Tensor memory: accumulators, then four 16-column scale slots.
-  static constexpr int NBUF = PAIR ? 1 : (2 * MB * BN + 64 <= 512 ? 2 : 1);  // accumulator barriers
-  static constexpr int ACC_COLS = PAIR ? 448 : NBUF * MB * BN;
+  // Tensor memory: accumulators, then four 16-column scale slots.  (Swapped tiles: at most half of it, so
+  // that a second block's allocation never has to wait for the first block.)
+  static constexpr int ACC_COLS = SWAP ? MB * BN : 448;
   static constexpr int SLOT_COLS = 16;
   static constexpr int TMEM_COLS = ACC_COLS + 64 <= 128 ? 128 : ACC_COLS + 64 <= 256 ? 256 : 512;
-  static_assert(ACC_COLS % 16 == 0 && ACC_COLS + 64 <= TMEM_COLS, "tensor memory");
-  static_assert(PAIR ? BN == 256 : (BN >= 16 && BN <= 128 && BN % 16 == 0), "tile shapes");
-  static_assert(STAGE_BYTES % 1024 == 0 && STAGES >= 4, "ring");
-  static_assert(PAIR || MB * BN * 128 * 4 <= RING_BYTES, "partial sums meet in the ring");
-  static_assert(8 * (2 * STAGES + 5) + 16 <= BAR_BYTES, "barriers");
+  static_assert(ACC_COLS % 16 == 0 && ACC_COLS + 64 <= TMEM_COLS && (!SWAP || TMEM_COLS <= 256), "tensor memory");
+  static_assert(SWAP ? (BN <= 64 && BN % 16 == 0 && CTAS == 1) : BN == 256, "tile shapes");
+  static_assert(STAGE_BYTES % 1024 == 0 && STAGES >= 2, "ring");
+  static_assert((SWAP ? MB * BN : 256) * 128 * 4 <= RING_BYTES, "partial sums meet in the ring");
+  static_assert(8 * (2 * STAGES + 3) + 16 <= BAR_BYTES, "barriers");
 };
 
 namespace detail {
@@ -147,13 +154,6 @@ __device__ __forceinline__ float mx_load_c(const MxParams& p, int64_t at) {
     case 0: return __half2float(static_cast<const __half*>(p.c)[at]);
     case 1: return __bfloat162float(static_cast<const __nv_bfloat16*>(p.c)[at]);
     default: return static_cast<const float*>(p.c)[at];
-  }
-}
-__device__ __forceinline__ void mx_store(const MxParams& p, int64_t at, float v) {
-  switch (p.out_type) {
-    case 0: static_cast<__half*>(p.d)[at] = __float2half_rn(v); break;
-    case 1: static_cast<__nv_bfloat16*>(p.d)[at] = __float2bfloat16_rn(v); break;
-    default: static_cast<float*>(p.d)[at] = v;
   }
 }
 
@@ -316,87 +316,124 @@ __device__ __forceinline__ void mx_store_quantized(const MxParams& p, const floa
         make_uint4(codes[0], codes[1], codes[2], codes[3]);
 }
 
-// One output row of a swapped tile, quantised: the warp's 32 lanes are 32 consecutive columns.
+// One output row of a swapped tile, quantised: the warp's lanes hold four neighbouring columns each, so
+// eight lanes share an e8m0 block and four an e4m3 block.
 template <bool NV>
-__device__ __forceinline__ void mx_store_quantized_lane(const MxParams& p, float h, uint32_t row, uint32_t col0,
-                                                        uint32_t lane) {
-  const float v = col0 + lane < p.n ? h * p.out_multiplier : 0.0f;
-  const uint32_t mask = NV ? (lane < 16u ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
-  // as integers the magnitudes order like the numbers, with NaN above infinity
-  const uint32_t top = __reduce_max_sync(mask, __float_as_uint(v) & 0x7FFFFFFFu);
-  const mx::Scale s = mx::block_scale<NV>(__uint_as_float(top));
-  uint32_t word = s.byte == mx::Format<NV>::NAN_SCALE ? 0u : mx::pack1(mx::in_code_units<NV>(v, s)) << (4u * (lane & 7u));
+__device__ __forceinline__ void mx_store_quantized_row(const MxParams& p, const float (&f)[4], uint32_t row, uint32_t col,
+                                                       uint32_t lane) {
+  constexpr int LANES = mx::Format<NV>::BLOCK / 4;
+  float v[4];
+  float amax = 0.0f;
 #pragma unroll
-  for (int d = 1; d < 8; d *= 2) word |= __shfl_xor_sync(0xFFFFFFFFu, word, d);
-  if ((lane & 7u) == 0u && col0 < p.n && GZ_MX_STORE_OK(p, row, col0, 1u, p.m, p.n))
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.d) + static_cast<int64_t>(row) * p.ldd + (col0 + lane) / 2) = word;
-  constexpr uint32_t BLOCK = mx::Format<NV>::BLOCK;
-  const int64_t block = (col0 + lane) / BLOCK;
-  if (lane % BLOCK == 0u && block < 4 * p.d_groups)
+  for (int i = 0; i < 4; ++i) {
+    v[i] = col + i < p.n ? f[i] * p.out_multiplier : 0.0f;
+    amax = mx::amax_nan(amax, v[i]);
+  }
+#pragma unroll
+  for (int d = 1; d < LANES; d *= 2) amax = mx::amax_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+  const mx::Scale s = mx::block_scale<NV>(amax);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mx::in_code_units<NV>(v[i], s);
+  uint32_t codes = mx::pack8(v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f);
+  if (s.byte == mx::Format<NV>::NAN_SCALE) codes = 0u;
+  if ((col & ~31u) < p.n && GZ_MX_STORE_OK(p, row, col & ~31u, 1u, p.m, p.n))  // the codes of a row fill up whole 32s
+    *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.d) + static_cast<int64_t>(row) * p.ldd + col / 2) =
+        static_cast<uint16_t>(codes);
+  const int64_t block = col / mx::Format<NV>::BLOCK;
+  if (lane % LANES == 0u && block < 4 * p.d_groups)
     p.d_scales[mx::scale_word(row, block >> 2, p.d_groups) + (block & 3)] = static_cast<uint8_t>(s.byte);
+}
+
+// Up to four columns of a row as fp32, and back (`n` of them exist).
+__device__ __forceinline__ void mx_load4(const float* v, uint32_t n, float (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = static_cast<uint32_t>(i) < n ? __ldg(v + i) : 0.0f;
 }
 
 }  // namespace detail
 
-// Finish up to N output rows row0, row0 + step, ... of a swapped tile: the lane is column col0 + lane,
-// f (and u) are the accumulators.  All 32 lanes take part.
-template <class Cfg, int N>
-__device__ __forceinline__ void mx_finish_rows(const MxParams& p, float (&f)[N], float (&u)[N], uint32_t row0,
-                                               uint32_t step, uint32_t count, uint32_t col0, uint32_t lane) {
-  const uint32_t col = col0 + lane;
-  const bool col_ok = col < p.n;
+// Finish one output row of a swapped tile: the warp's lanes hold the sums of four neighbouring columns each.
+template <class Cfg>
+__device__ __forceinline__ void mx_finish_row(const MxParams& p, float (&f)[4], const float (&u)[4], uint32_t row,
+                                              uint32_t col, uint32_t lane) {
+  const uint32_t have = col >= p.n ? 0u : p.n - col < 4u ? p.n - col : 4u;  // columns that exist
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] *= p.alpha;
+  for (int i = 0; i < 4; ++i) f[i] *= p.alpha;
   if constexpr (Cfg::GATED) {
     detail::activate_all(f, p.act);
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] *= p.alpha_up * u[i];
-    if (p.out_type >= MX_OUT_FP4) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (static_cast<uint32_t>(i) >= count) break;
-        if (p.out_type == MX_OUT_FP4) detail::mx_store_quantized_lane<false>(p, f[i], row0 + i * step, col0, lane);
-        else detail::mx_store_quantized_lane<true>(p, f[i], row0 + i * step, col0, lane);
-      }
-      return;
-    }
-  } else {
+    for (int i = 0; i < 4; ++i) f[i] *= p.alpha_up * u[i];
+    if (p.out_type == MX_OUT_FP4) return detail::mx_store_quantized_row<false>(p, f, row, col, lane);
+    if (p.out_type == MX_OUT_NVFP4) return detail::mx_store_quantized_row<true>(p, f, row, col, lane);
+  }
+  if (have == 0u || !GZ_MX_STORE_OK(p, row, col, have, p.m, p.n)) return;
+  const bool vec = have == 4u && p.d_vec_ok;
+  if constexpr (!Cfg::GATED) {
+    float t[4];
     if (p.epi_flags & 2u) {
+      const float rs = __ldg(p.row_scale + row);
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (static_cast<uint32_t>(i) < count) f[i] *= __ldg(p.row_scale + row0 + i * step);
+      for (int i = 0; i < 4; ++i) f[i] *= rs;
     }
     if (p.epi_flags & 4u) {
-      const float cs = col_ok ? __ldg(p.col_scale + col) : 1.0f;
+      detail::mx_load4(p.col_scale + col, have, t);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= cs;
+      for (int i = 0; i < 4; ++i) f[i] *= t[i];
     }
-    if (p.beta != 0.0f && col_ok) {
+    if (p.beta != 0.0f) {
+      const int64_t at = static_cast<int64_t>(row) * p.ldc + col;
+      if (vec && p.out_type != 2u) {
+        const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.c) + at);
+        const float2 lo = p.out_type == 0u ? detail::unpack2<__half>(w.x) : detail::unpack2<__nv_bfloat16>(w.x);
+        const float2 hi = p.out_type == 0u ? detail::unpack2<__half>(w.y) : detail::unpack2<__nv_bfloat16>(w.y);
+        t[0] = lo.x;
+        t[1] = lo.y;
+        t[2] = hi.x;
+        t[3] = hi.y;
+      } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (static_cast<uint32_t>(i) < count)
-          f[i] = fmaf(p.beta, detail::mx_load_c(p, static_cast<int64_t>(row0 + i * step) * p.ldc + col), f[i]);
+        for (int i = 0; i < 4; ++i) t[i] = static_cast<uint32_t>(i) < have ? detail::mx_load_c(p, at + i) : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = fmaf(p.beta, t[i], f[i]);
     }
     if (p.epi_flags & 1u) {
-      const float b = col_ok ? __ldg(p.bias + col) : 0.0f;
+      detail::mx_load4(p.bias + col, have, t);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] += b;
+      for (int i = 0; i < 4; ++i) f[i] += t[i];
     }
     detail::activate_all(f, p.act);
   }
-  if (!col_ok) return;
+  const int64_t at = static_cast<int64_t>(row) * p.ldd + col;
+  if (p.out_type == 2u) {
+    float* d = static_cast<float*>(p.d) + at;
+    if (vec) {
+      *reinterpret_cast<float4*>(d) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (static_cast<uint32_t>(i) < count && GZ_MX_STORE_OK(p, row0 + i * step, col, 1u, p.m, p.n))
-      detail::mx_store(p, static_cast<int64_t>(row0 + i * step) * p.ldd + col, f[i]);
+      for (int i = 0; i < 4; ++i)
+        if (static_cast<uint32_t>(i) < have) d[i] = f[i];
+    }
+  } else {
+    uint2 w;
+    w.x = p.out_type == 0u ? detail::pack2<__half>(f[0], f[1]) : detail::pack2<__nv_bfloat16>(f[0], f[1]);
+    w.y = p.out_type == 0u ? detail::pack2<__half>(f[2], f[3]) : detail::pack2<__nv_bfloat16>(f[2], f[3]);
+    uint16_t* d = static_cast<uint16_t*>(p.d) + at;
+    if (vec) {
+      *reinterpret_cast<uint2*>(d) = w;
+    } else {
+      const uint32_t h[2] = {w.x, w.y};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (static_cast<uint32_t>(i) < have) d[i] = static_cast<uint16_t>(h[i >> 1] >> (16 * (i & 1)));
+    }
+  }
 }
 
 // Quantised output of a swapped tile: the scale rows from m up to the next multiple of 128 are zero.
-// `thread` (0..127) takes row 128 * group + thread of the tile's one (e8m0) or two (e4m3) scale tiles.
-__device__ __forceinline__ void mx_clear_scale_rows(const MxParams& p, uint32_t tm, uint32_t group, uint32_t thread) {
-  if (p.out_type < MX_OUT_FP4) return;
-  const uint32_t row = group * 128u + thread;
-  if (row < p.m) return;
+// `row` is one of the tile's 128 in its one (e8m0) or two (e4m3) scale tiles.
+__device__ __forceinline__ void mx_clear_scale_row(const MxParams& p, uint32_t tm, uint32_t row) {
+  if (p.out_type < MX_OUT_FP4 || row < p.m) return;
   const uint32_t words = p.out_type == MX_OUT_NVFP4 ? 2u : 1u;
   for (uint32_t w = 0; w < words; ++w) {
     const int64_t g = static_cast<int64_t>(tm) * words + w;
@@ -404,11 +441,38 @@ __device__ __forceinline__ void mx_clear_scale_rows(const MxParams& p, uint32_t 
   }
 }
 
+// 32 columns of one row (lane = row) of a row tile, from the sums to the output.
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::THREADS, 1)
+__device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* tm_d, uint32_t stg, uint32_t lane,
+                                                const uint32_t (&x)[32], const uint32_t (&y)[32], uint32_t row0,
+                                                uint32_t col0, uint32_t& turn) {
+  float f[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = p.alpha * __uint_as_float(x[i]);
+  if constexpr (Cfg::GATED) {
+    detail::activate_all(f, p.act);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] *= p.alpha_up * __uint_as_float(y[i]);
+    if (p.out_type >= MX_OUT_FP4) {
+      if (row0 < ((p.m + 127u) & ~127u)) {  // rows up to the next multiple of 128 have scales
+        if (p.out_type == MX_OUT_FP4) detail::mx_store_quantized<false>(p, f, row0 + lane, col0);
+        else detail::mx_store_quantized<true>(p, f, row0 + lane, col0);
+      }
+      return;
+    }
+    if (row0 >= p.m || col0 >= p.n) return;
+  } else {
+    if (row0 >= p.m || col0 >= p.n) return;
+    if (p.epi_flags != 0u || p.beta != 0.0f || p.act != 0u) detail::mx_row_terms(p, f, row0 + lane, col0, lane);
+  }
+  detail::mx_store_box(p, tm_d, stg, lane, f, row0, col0, turn);
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, Cfg::SWAP ? 2 : 1)
 mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
-  constexpr int CTAS = Cfg::CTAS, STAGES = Cfg::STAGES, BN = Cfg::BN, MB = Cfg::MB, NBUF = Cfg::NBUF;
-  constexpr bool NV = Cfg::NV, PAIR = Cfg::PAIR, GATED = Cfg::GATED;
+  constexpr int CTAS = Cfg::CTAS, STAGES = Cfg::STAGES, BN = Cfg::BN, MB = Cfg::MB;
+  constexpr bool NV = Cfg::NV, SWAP = Cfg::SWAP, GATED = Cfg::GATED;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
@@ -418,16 +482,18 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
   const uint32_t bars = staging_base + Cfg::STAGING_BYTES;
   auto full_bar = [&](uint32_t s) { return bars + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bars + 8u * (STAGES + s); };
-  auto acc_full_bar = [&](uint32_t b) { return bars + 8u * (2 * STAGES + b); };
-  auto acc_empty_bar = [&](uint32_t b) { return bars + 8u * (2 * STAGES + 2 + b); };
-  const uint32_t drain_bar = bars + 8u * (2 * STAGES + 4);
+  const uint32_t acc_full_bar = bars + 8u * (2 * STAGES), acc_empty_bar = acc_full_bar + 8u;
+  const uint32_t drain_bar = acc_full_bar + 16u;
   uint32_t* const tmem_slot =
-      reinterpret_cast<uint32_t*>(smem + Cfg::RING_BYTES + Cfg::STAGING_BYTES + 8 * (2 * STAGES + 5));
+      reinterpret_cast<uint32_t*>(smem + Cfg::RING_BYTES + Cfg::STAGING_BYTES + 8 * (2 * STAGES + 3));
   uint32_t* const abort_flag = tmem_slot + 1;
 
   const uint32_t warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
-  const uint32_t rank = ptx::cluster_ctarank();  // of the pair, or of the cluster that shares a K range
+  const uint32_t crank = ptx::cluster_ctarank();
+  const uint32_t rank = CTAS == 2 ? (crank & 1u) : 0u;  // within the pair
+  const uint32_t part = CTAS == 2 ? crank >> 1 : crank;  // which share of a tile's K range
+  const uint32_t leader = CTAS == 2 ? (crank & ~1u) : crank;
   const uint32_t cluster = ptx::cluster_id_x(), num_clusters = ptx::num_clusters_x();
   const detail::Abort ab{abort_flag, p.status, p.wait_limit_ns};
 
@@ -440,11 +506,9 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
       ptx::mbar_init(full_bar(s), 2);
       ptx::mbar_init(empty_bar(s), 1);
     }
-    if (lane < 2u) {
-      ptx::mbar_init(acc_full_bar(lane), 1);
-      ptx::mbar_init(acc_empty_bar(lane), Cfg::EPI_WARPS * CTAS);
-    }
-    if (lane == 2u) {
+    if (lane == 0u) {
+      ptx::mbar_init(acc_full_bar, 1);
+      ptx::mbar_init(acc_empty_bar, Cfg::EPI_WARPS * CTAS);
       ptx::mbar_init(drain_bar, 1);
       *abort_flag = 0u;
     }
@@ -474,13 +538,12 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   ptx::grid_launch_dependents();
 
-  // The tiles of this cluster and the K blocks of each that are this CTA's.
+  // The K blocks that are this CTA's (pair's).  The tiles: a swapped CTA has one; a row-tile cluster that
+  // shares K ranges has one; otherwise a cluster is a CTA (pair) that walks tiles in steps of the grid.
   uint32_t kb_lo = 0, kb_hi = p.k_blocks;
-  if constexpr (!PAIR) {
-    if (p.split > 1u) {
-      kb_lo = static_cast<uint32_t>(static_cast<uint64_t>(rank) * p.k_blocks / p.split);
-      kb_hi = static_cast<uint32_t>(static_cast<uint64_t>(rank + 1u) * p.k_blocks / p.split);
-    }
+  if (p.split > 1u) {
+    kb_lo = static_cast<uint32_t>(static_cast<uint64_t>(part) * p.k_blocks / p.split);
+    kb_hi = static_cast<uint32_t>(static_cast<uint64_t>(part + 1u) * p.k_blocks / p.split);
   }
 
   if (warp == 0 || warp == 6) {
@@ -494,20 +557,25 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
     for (uint32_t t = cluster; ok && t < p.grid.num_tiles; t += num_clusters) {
       uint32_t tm, tn;
       tile_coords(p.grid, t, tm, tn);
-      const int32_t wide_rb = static_cast<int32_t>(PAIR ? tm * 2u + rank : tm);
+      const int32_t wide_rb = static_cast<int32_t>(tm * CTAS + rank);
+      // Swapped tiles stream B once: they start at different K blocks, or all CTAs would read addresses a
+      // multiple of the row pitch apart, which load the HBM channels unevenly.
+      const uint32_t rot = SWAP ? (t * 5u) % (kb_hi - kb_lo) : 0u;
       for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
         ok = __all_sync(0xFFFFFFFFu, detail::wait(empty_bar(stage), phase ^ 1u, ab, WAIT_PRODUCER_EMPTY, t, kb));
         if (!ok) break;
         if (ptx::elect_one()) {
           const uint32_t dst = base + stage * Cfg::STAGE_BYTES;
-          const int32_t kx = static_cast<int32_t>(kb * 128u);
-          const int32_t kt = static_cast<int32_t>(kb * Cfg::TILES_K);
+          uint32_t at = kb + rot;  // K block fetched in this step
+          if (at >= kb_hi) at -= kb_hi - kb_lo;
+          const int32_t kx = static_cast<int32_t>(at * 128u);
+          const int32_t kt = static_cast<int32_t>(at * Cfg::TILES_K);
           uint32_t fb = full_bar(stage);
           if constexpr (CTAS == 1) {
             ptx::mbar_arrive_expect_tx(fb, my_bytes);
           } else {
             if (rank == 0) ptx::mbar_arrive_expect_tx(fb, 2u * my_bytes);
-            fb = ptx::mapa(fb, 0);
+            fb = ptx::mapa(fb, leader);
           }
           auto load = [&](uint32_t to, const void* map, int32_t c0, int32_t c1, int32_t c2) {
             if constexpr (CTAS == 1) ptx::tma_load_3d(to, map, c0, c1, c2, fb);
@@ -521,17 +589,20 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
               load(dst + 128u * 128u, &maps.up, kx, wide_rb * 128, 0);
               load(ws + Cfg::TILES_K * 512u, &maps.up_scales, 0, kt, wide_rb);
             }
-          } else if constexpr (PAIR) {
-            const int32_t rb0 = static_cast<int32_t>(GATED ? tn : tn * 2u);
+          } else if constexpr (!SWAP) {
+            // 256 rows as two groups of 128: rows of B, or the gate's and the up projection's
+            const int32_t rb0 = static_cast<int32_t>(GATED ? tn : tn * 2u), rb1 = GATED ? rb0 : rb0 + 1;
+            const CUtensorMap* const second = GATED ? &maps.up : &maps.narrow;
             const CUtensorMap* const second_scales = GATED ? &maps.up_scales : &maps.narrow_scales;
-            const int32_t rb1 = GATED ? rb0 : rb0 + 1;
-            load(dst + Cfg::W_BYTES, (GATED && rank == 1u) ? &maps.up : &maps.narrow, kx,
-                 (rank == 0u ? rb0 : rb1) * 128, 0);
+            const uint32_t nd = dst + Cfg::W_BYTES;
+            if (CTAS == 1 || rank == 0u) load(nd, &maps.narrow, kx, rb0 * 128, 0);
+            if (CTAS == 1) load(nd + 128u * 128u, second, kx, rb1 * 128, 0);
+            else if (rank == 1u) load(nd, second, kx, rb1 * 128, 0);
             load(ns, &maps.narrow_scales, 0, kt, rb0);
             load(ns + Cfg::TILES_K * 512u, second_scales, 0, kt, rb1);
           } else {
-            load(dst + Cfg::W_BYTES, &maps.narrow, kx, static_cast<int32_t>(tn * BN), 0);
-            load(ns, &maps.narrow_scales, 0, kt, static_cast<int32_t>(tn * BN / 128u));
+            load(dst + Cfg::W_BYTES, &maps.narrow, kx, 0, 0);
+            load(ns, &maps.narrow_scales, 0, kt, 0);
           }
         }
         __syncwarp();
@@ -555,7 +626,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     ptx::grid_dependency_wait();
-    if (!PAIR || rank == 0) {
+    if (rank == 0) {
       uint32_t stage = 0, phase = 0, it = 0, slot = 0;
       bool ok = true, issued = false;
       // Shared-memory descriptors: codes in 128-byte-swizzled rows (8 rows = 1024 bytes); scales as
@@ -563,17 +634,10 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
       const uint64_t code_hi = static_cast<uint64_t>((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | (1u << 16);
       const uint64_t scale_hi = static_cast<uint64_t>((128u >> 4) | (1u << 14)) << 32 | ((128u >> 4) << 16);
       for (uint32_t t = cluster; ok && t < p.grid.num_tiles; t += num_clusters, ++it) {
-        const uint32_t buf = it % NBUF;
-        ok = __all_sync(0xFFFFFFFFu, detail::wait(acc_empty_bar(buf), ((it / NBUF) & 1u) ^ 1u, ab, WAIT_MMA_TMEM_EMPTY, t, 0));
+        ok = __all_sync(0xFFFFFFFFu, detail::wait(acc_empty_bar, (it & 1u) ^ 1u, ab, WAIT_MMA_TMEM_EMPTY, t, 0));
         if (!ok) break;
         ptx::tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + (PAIR ? (it & 1u) * 192u : buf * (MB * BN));
-        uint32_t narrow_off = 0;  // scale columns of the narrow tile's first row within its group of 128
-        if constexpr (!PAIR && BN < 128) {
-          uint32_t tm, tn;
-          tile_coords(p.grid, t, tm, tn);
-          narrow_off = (tn * BN % 128u) / 32u;
-        }
+        const uint32_t d_tmem = tmem_base + (SWAP ? 0u : (it & 1u) * 192u);
         for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
           ok = __all_sync(0xFFFFFFFFu, detail::wait(full_bar(stage), phase, ab, WAIT_MMA_FULL, t, kb));
           if (!ok) break;
@@ -600,11 +664,11 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
 #pragma unroll
                 for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb)
                   ptx::umma_mx<NV, CTAS>(d_tmem + mb * BN, wd + step * 2u + mb * ((128u * 128u) >> 4), nd + step * 2u,
-                                         idesc, sf + mb * 4u, sf + 8u + narrow_off, (kb != kb_lo || step != 0u) ? 1u : 0u);
+                                         idesc, sf + mb * 4u, sf + 8u, (kb != kb_lo || step != 0u) ? 1u : 0u);
               }
             }
             ptx::tc_commit<CTAS>(empty_bar(stage));
-            if constexpr (CTAS == 2) ptx::tc_commit<CTAS>(ptx::mapa(empty_bar(stage), 1));
+            if constexpr (CTAS == 2) ptx::tc_commit<CTAS>(ptx::mapa(empty_bar(stage), crank | 1u));
           }
           __syncwarp();
           issued = true;
@@ -616,8 +680,8 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
         }
         if (!ok) break;
         if (!(p.test_flags & 1u) && ptx::elect_one()) {
-          ptx::tc_commit<CTAS>(acc_full_bar(buf));
-          if constexpr (CTAS == 2) ptx::tc_commit<CTAS>(ptx::mapa(acc_full_bar(buf), 1));
+          ptx::tc_commit<CTAS>(acc_full_bar);
+          if constexpr (CTAS == 2) ptx::tc_commit<CTAS>(ptx::mapa(acc_full_bar, crank | 1u));
         }
         __syncwarp();
       }
@@ -634,19 +698,52 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
     ptx::grid_dependency_wait();
     const uint32_t quad = warp & 3u;
     const uint32_t lanes = tmem_base + ((quad * 32u) << 16);
-    uint32_t it = 0;
-    if constexpr (PAIR) {
+    // Partial (or whole) sums in shared memory: [column of the accumulator][128 lanes].
+    const uint32_t park = base + (quad * 32u + lane) * 4u;
+    if constexpr (SWAP) {
+      if (cluster < p.grid.num_tiles && detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0)) {
+        ptx::tc_fence_after_sync();
+#pragma unroll 1
+        for (uint32_t sl = 0; sl * 16u < p.m; ++sl) {
+          uint32_t x[MB][16];
+#pragma unroll
+          for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb) ptx::tmem_ld_32x16(lanes + mb * BN + sl * 16u, x[mb]);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb) {
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(park + (mb * BN + sl * 16u + i) * 512u), "r"(x[mb][i]) : "memory");
+          }
+        }
+        ptx::tc_fence_before_sync();
+      }
+    } else {
       const uint32_t half = warp >= 7u ? 1u : 0u;
       const uint32_t stg = staging_base + (half * 4u + quad) * 4096u;
-      const uint32_t release = ptx::mapa(acc_empty_bar(0), 0);
-      uint32_t turn = 0;
+      const uint32_t release = ptx::mapa(acc_empty_bar, leader);
+      uint32_t turn = 0, it = 0;
       for (uint32_t t = cluster; t < p.grid.num_tiles; t += num_clusters, ++it) {
         uint32_t tm, tn;
         tile_coords(p.grid, t, tm, tn);
-        const uint32_t row0 = tm * 256u + rank * 128u + quad * 32u;
-        if (!detail::wait(acc_full_bar(0), it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
+        const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
+        if (!detail::wait(acc_full_bar, it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
         ptx::tc_fence_after_sync();
         const uint32_t acc = lanes + (it & 1u) * 192u;
+        if (p.split > 1u) {
+#pragma unroll 1
+          for (uint32_t g = 0; g < 4u; ++g) {
+            const uint32_t off = g * 64u + half * 32u;
+            uint32_t x[32];
+            ptx::tmem_ld_32x32(acc + off, x);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(park + (off + i) * 512u), "r"(x[i]) : "memory");
+          }
+          ptx::tc_fence_before_sync();
+          break;  // the cluster's only tile
+        }
         constexpr uint32_t GROUPS = GATED ? 2u : 4u;  // of 64 columns; this warp's half of each is 32 wide
 #pragma unroll 1
         for (uint32_t s = 0; s < GROUPS; ++s) {
@@ -662,112 +759,100 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_cluster(release);
           }
-          const uint32_t col0 = tn * (GATED ? 128u : 256u) + off;
-          float f[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = p.alpha * __uint_as_float(x[i]);
-          if constexpr (GATED) {
-            detail::activate_all(f, p.act);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] *= p.alpha_up * __uint_as_float(y[i]);
-            if (p.out_type >= MX_OUT_FP4) {
-              if (row0 < ((p.m + 127u) & ~127u)) {
-                if (p.out_type == MX_OUT_FP4) detail::mx_store_quantized<false>(p, f, row0 + lane, col0);
-                else detail::mx_store_quantized<true>(p, f, row0 + lane, col0);
-              }
-              continue;
-            }
-            if (row0 >= p.m || col0 >= p.n) continue;
-          } else {
-            if (row0 >= p.m || col0 >= p.n) continue;
-            if (p.epi_flags != 0u || p.beta != 0.0f || p.act != 0u) detail::mx_row_terms(p, f, row0 + lane, col0, lane);
-          }
-          detail::mx_store_box(p, &maps.d, stg, lane, f, row0, col0, turn);
+          mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, row0, tn * (GATED ? 128u : 256u) + off, turn);
         }
-        // the barrier counts one release per tile, made above; the rest of this tile's columns are read
-        // before the next tile's release, which is what the tile after that waits for
+        // one release per tile, made above; the rest of this tile's columns are read before the next
+        // tile's release, which is what the tile after that waits for
         ptx::tc_fence_before_sync();
       }
-      if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
-    } else {
-      const uint32_t feature_in_tile = quad * 32u + lane;
-      for (uint32_t t = cluster; t < p.grid.num_tiles; t += num_clusters, ++it) {
-        uint32_t tm, tn;
-        tile_coords(p.grid, t, tm, tn);
-        const uint32_t buf = it % NBUF;
-        if (!detail::wait(acc_full_bar(buf), (it / NBUF) & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
-        ptx::tc_fence_after_sync();
-        const uint32_t acc = lanes + buf * (MB * BN);
-        const uint32_t token0 = tn * BN;
-        const uint32_t tokens = p.m - token0 < static_cast<uint32_t>(BN) ? p.m - token0 : static_cast<uint32_t>(BN);
-#pragma unroll 1
-        for (uint32_t sl = 0; sl * 16u < tokens; ++sl) {
-          uint32_t x[16], y[16];
-          ptx::tmem_ld_32x16(acc + sl * 16u, x);
-          if constexpr (GATED) ptx::tmem_ld_32x16(acc + BN + sl * 16u, y);
-          ptx::tmem_wait_ld();
-          if (p.split > 1u) {
-            // Park the partial sums: [operand][row of A][128 features].
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-              const uint32_t at = base + ((sl * 16u + i) * 128u + feature_in_tile) * 4u;
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x[i]) : "memory");
-              if constexpr (GATED)
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + BN * 512u), "r"(y[i]) : "memory");
-            }
-          } else {
-            float f[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(x[i]);
-            float u[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = GATED ? __uint_as_float(y[i]) : 0.0f;
-            const uint32_t count = tokens - sl * 16u < 16u ? tokens - sl * 16u : 16u;
-            mx_finish_rows<Cfg, 16>(p, f, u, token0 + sl * 16u, 1u, count, tm * 128u + quad * 32u, lane);
-          }
-        }
-        if (p.split <= 1u) {
-          if constexpr (GATED) mx_clear_scale_rows(p, tm, token0 / 128u, (warp & 3u) * 32u + lane);
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(acc_empty_bar(buf));
-        }
-      }
+      if (p.split <= 1u && p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
     }
   }
 
-  // -------------------------------------------------------------- shared K range: add the partial sums
-  if constexpr (!PAIR) {
+  // -------------------------------------------------------------- sums that met in shared memory
+  if (SWAP || p.split > 1u) {
+    __syncwarp();
     if (p.split > 1u) {
-      __syncwarp();
       ptx::cluster_arrive_release();
       ptx::cluster_wait_acquire();
-      const bool epilogue = warp >= 2u && warp != 6u;
-      if (epilogue && cluster < p.grid.num_tiles && !detail::aborted(ab)) {
-        uint32_t tm, tn;
-        tile_coords(p.grid, cluster, tm, tn);
-        const uint32_t quad = warp & 3u;
-        const uint32_t token0 = tn * BN;
-        const uint32_t tokens = p.m - token0 < static_cast<uint32_t>(BN) ? p.m - token0 : static_cast<uint32_t>(BN);
-        const uint32_t mine = base + (quad * 32u + lane) * 4u;
-        // rows rank, rank + split, ... of the tile, four at a time
-        for (uint32_t r = rank; r < tokens; r += 4u * p.split) {
-          float f[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint32_t count = (tokens - r + p.split - 1u) / p.split < 4u ? (tokens - r + p.split - 1u) / p.split : 4u;
-          for (uint32_t q = 0; q < p.split; ++q) {
-            const uint32_t peer = ptx::mapa(mine, q);
+    } else {
+      __syncthreads();
+    }
+    if (cluster < p.grid.num_tiles && !detail::aborted(ab)) {
+      uint32_t tm, tn;
+      tile_coords(p.grid, cluster, tm, tn);
+      if constexpr (SWAP) {
+        // Output rows part, part + split, ... dealt to the block's warps.
+        const uint32_t mine = base + lane * 16u;
+        const uint32_t col = tm * 128u + lane * 4u;
+        for (uint32_t r = part + p.split * warp; r < p.m; r += p.split * (Cfg::THREADS / 32)) {
+          float f[4] = {}, u[4] = {};
+          if (p.split == 1u) {
+            ptx::ld_shared_f32x4(mine + r * 512u, f);
+            if constexpr (GATED) ptx::ld_shared_f32x4(mine + (BN + r) * 512u, u);
+          } else {
+            for (uint32_t q = 0; q < p.split; q += 2u) {  // two peers' loads in flight
+              const uint32_t a0 = ptx::mapa(mine, q) + r * 512u, a1 = ptx::mapa(mine, q + 1u) + r * 512u;
+              float x0[4], x1[4], y0[4], y1[4];
+              ptx::ld_cluster_f32x4(a0, x0);
+              ptx::ld_cluster_f32x4(a1, x1);
+              if constexpr (GATED) {
+                ptx::ld_cluster_f32x4(a0 + BN * 512u, y0);
+                ptx::ld_cluster_f32x4(a1 + BN * 512u, y1);
+              }
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-              if (i >= count) break;
-              const uint32_t at = peer + (r + i * p.split) * 512u;
-              f[i] += ptx::ld_cluster_f32(at);
-              if constexpr (GATED) u[i] += ptx::ld_cluster_f32(at + BN * 512u);
+              for (int i = 0; i < 4; ++i) {
+                f[i] = (f[i] + x0[i]) + x1[i];
+                if constexpr (GATED) u[i] = (u[i] + y0[i]) + y1[i];
+              }
             }
           }
-          mx_finish_rows<Cfg, 4>(p, f, u, token0 + r, p.split, count, tm * 128u + quad * 32u, lane);
+          mx_finish_row<Cfg>(p, f, u, r, col, lane);
         }
-        if (GATED && rank == 0) mx_clear_scale_rows(p, tm, token0 / 128u, (warp & 3u) * 32u + lane);
+        if constexpr (GATED) {
+          if (part == 0u)
+            for (uint32_t r = threadIdx.x; r < 128u; r += Cfg::THREADS) mx_clear_scale_row(p, tm, r);
+        }
+      } else if (warp >= 2u && warp != 6u) {
+        // The tile's 32-column slices are dealt to the parts in order; a slice is finished by the warps of
+        // one half, as without a shared K range.
+        const uint32_t quad = warp & 3u, half = warp >= 7u ? 1u : 0u;
+        const uint32_t stg = staging_base + (half * 4u + quad) * 4096u;
+        const uint32_t mine = base + (quad * 32u + lane) * 4u;
+        const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
+        constexpr uint32_t SLICES = GATED ? 4u : 8u;
+        uint32_t turn = 0;
+        for (uint32_t sl = part * SLICES / p.split; sl < (part + 1u) * SLICES / p.split; ++sl) {
+          if ((sl & 1u) != half) continue;
+          float f[32], u[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = u[i] = 0.0f;
+          for (uint32_t q = 0; q < p.split; ++q) {
+            const uint32_t peer = ptx::mapa(mine, CTAS == 2 ? q * 2u + rank : q) + sl * 32u * 512u;
+            float x[32];
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) x[i] = ptx::ld_cluster_f32(peer + i * 512u);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] += x[i];
+            if constexpr (GATED) {
+#pragma unroll
+              for (uint32_t i = 0; i < 32; ++i) x[i] = ptx::ld_cluster_f32(peer + (128u + i) * 512u);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) u[i] += x[i];
+            }
+          }
+          uint32_t x[32], y[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            x[i] = __float_as_uint(f[i]);
+            y[i] = __float_as_uint(u[i]);
+          }
+          mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, row0, tn * (GATED ? 128u : 256u) + sl * 32u, turn);
+        }
+        if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
       }
+    }
+    if (p.split > 1u) {
       __syncwarp();
       ptx::cluster_arrive_release();  // nobody leaves while a peer may still read its partial sums
       ptx::cluster_wait_acquire();

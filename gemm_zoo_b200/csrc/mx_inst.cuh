@@ -37,10 +37,10 @@ cudaError_t mx_launch(const MxMaps& maps, const MxParams& p, int grid, int clust
   return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<Cfg>, maps, p);
 }
 
-template <bool NV, int BN, bool PAIR>
+template <bool NV, int BN, int CTAS>
 MxEntry mx_entry(bool gated) {
-  using G = MxCfg<NV, BN, PAIR, true>;
-  using P = MxCfg<NV, BN, PAIR, false>;
+  using G = MxCfg<NV, BN, CTAS, true>;
+  using P = MxCfg<NV, BN, CTAS, false>;
   if (gated) return {mx_launch<G>, mx_set_attr<G>, G::STAGES, G::SMEM_BYTES};
   return {mx_launch<P>, mx_set_attr<P>, P::STAGES, P::SMEM_BYTES};
 }
@@ -48,11 +48,11 @@ MxEntry mx_entry(bool gated) {
 template <bool NV>
 MxEntry mx_entry_for(int config, bool gated) {
   switch (config) {
-    case GZ_MX_CFG_PAIR: return mx_entry<NV, 256, true>(gated);
-    case GZ_MX_CFG_SWAP_M16: return mx_entry<NV, 16, false>(gated);
-    case GZ_MX_CFG_SWAP_M32: return mx_entry<NV, 32, false>(gated);
-    case GZ_MX_CFG_SWAP_M64: return mx_entry<NV, 64, false>(gated);
-    case GZ_MX_CFG_SWAP_M128: return mx_entry<NV, 128, false>(gated);
+    case GZ_MX_CFG_PAIR: return mx_entry<NV, 256, 2>(gated);
+    case GZ_MX_CFG_SINGLE: return mx_entry<NV, 256, 1>(gated);
+    case GZ_MX_CFG_SWAP_M16: return mx_entry<NV, 16, 1>(gated);
+    case GZ_MX_CFG_SWAP_M32: return mx_entry<NV, 32, 1>(gated);
+    case GZ_MX_CFG_SWAP_M64: return mx_entry<NV, 64, 1>(gated);
   }
   return {nullptr, nullptr, 0, 0};
 }

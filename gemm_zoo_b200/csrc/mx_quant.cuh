@@ -7,6 +7,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "mx_format.cuh"
 #include "ptx.cuh"
 
@@ -21,9 +23,11 @@ struct QuantParams {
   int64_t rows, k, ld, pitch;
   int64_t code_bytes;  // of a row: round_up(k, 32) / 2
   int64_t groups;      // scale tiles per 128 rows
-  int64_t items;       // work items of the launch (row layout)
-  uint32_t per_row;    // 16-element chunks per row, a whole number of scale words
-  uint32_t vec;        // vector access to the values is legal
+  // Row layout: a block takes `block_rows` rows x `row_threads` 16-element chunks (a whole number of
+  // scale words); inv_threads = ceil(65536 / row_threads) divides a thread index by row_threads.
+  uint32_t row_threads, inv_threads, block_rows;
+  uint32_t vec;   // vector access to the values is legal
+  uint32_t unit;  // multiplier == 1
   float multiplier;
 };
 
@@ -57,240 +61,327 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
-// Which (row, chunk) the thread's item is: the block's first item is divided in 64 bits once, the
-// thread's offset from it in 32.
-__device__ __forceinline__ void item_coords(const QuantParams& p, int64_t first, uint32_t offset, int64_t& row,
-                                            uint32_t& chunk) {
-  const int64_t row0 = first / p.per_row;
-  const uint32_t rem = static_cast<uint32_t>(first - row0 * p.per_row) + offset;
-  const uint32_t add = rem / p.per_row;
-  row = row0 + add;
-  chunk = rem - add * p.per_row;
-}
-
-// Rows with K contiguous.  A thread takes 16 consecutive elements (32 bytes of a 16-bit type in one
-// load), which is one e4m3 block or half of an e8m0 block; the lanes that share a 4-byte word of
-// scales are neighbours, so amax and the word are put together with shuffles.  Rows beyond the last
-// up to the next multiple of 128 exist in the scale array only and get zero bytes.
-template <typename T, bool NV>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p) {
-  constexpr int PER_WORD = NV ? 4 : 8;  // threads whose blocks share a word of scales
-  ptx::grid_launch_dependents();
-  ptx::grid_dependency_wait();
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x;
-  const bool mine = first + threadIdx.x < p.items;
-  const uint32_t mask = __ballot_sync(0xFFFFFFFFu, mine);  // whole words: items are a multiple of PER_WORD
-  if (!mine) return;
-  int64_t row;
-  uint32_t chunk;
-  item_coords(p, first, threadIdx.x, row, chunk);
-  const int64_t k0 = static_cast<int64_t>(chunk) * 16;
-  float v[16];
-  const T* src = static_cast<const T*>(p.in) + row * p.ld + k0;
-  if (row < p.rows && k0 + 16 <= p.k && p.vec) {
-    constexpr int LOADS = sizeof(T) / 2;
+// Largest magnitude among 16 values held as raw bits, as raw bits (of one value): without their signs
+// the numbers order like integers, NaN above infinity.
+template <typename T>
+__device__ __forceinline__ float amax_raw(const uint32_t* w) {
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 2) {
+    uint32_t a[8];
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-      uint32_t w[8];
-      load32(src + l * (16 / LOADS), w);
-      const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-      for (int i = 0; i < 16 / LOADS; ++i) v[l * (16 / LOADS) + i] = to_float<T>(e[i]);
-    }
+    for (int i = 0; i < 8; ++i) a[i] = w[i] & 0x7FFF7FFFu;
+    m = __vimax3_u16x2(__vimax3_u16x2(a[0], a[1], a[2]), __vimax3_u16x2(a[3], a[4], a[5]), __vimax3_u16x2(a[6], a[7], 0u));
+    m = max(m & 0xFFFFu, m >> 16);
+    const uint16_t h = static_cast<uint16_t>(m);
+    return to_float<T>(*reinterpret_cast<const T*>(&h));
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = (row < p.rows && k0 + i < p.k) ? to_float<T>(src[i]) : 0.0f;
+    for (int i = 0; i < 16; i += 2) m = __vimax3_u32(m, w[i] & 0x7FFFFFFFu, w[i + 1] & 0x7FFFFFFFu);
+    return __uint_as_float(m);
   }
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    v[i] *= p.multiplier;
-    amax = amax_nan(amax, v[i]);
+}
+
+// Value i of a row of raw words.
+template <typename T>
+__device__ __forceinline__ float value_of(const uint32_t* w, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+  else {
+    const uint16_t h = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+    return __half2float(*reinterpret_cast<const __half*>(&h));
   }
+}
+
+// 16 raw values of one row -> their 8 bytes of codes; `scale` receives the byte of their block.  An e8m0
+// block is shared with the neighbouring lane (`mask`: the lanes that call).  The largest magnitude is
+// taken before the multiplier, which rounding, being monotone, allows.
+template <typename T, bool NV>
+__device__ __forceinline__ uint2 encode16(const uint32_t* w, const QuantParams& p, uint32_t mask, uint32_t& scale) {
+  float amax = amax_raw<T>(w) * fabsf(p.multiplier);
   if constexpr (!NV) amax = amax_nan(amax, __shfl_xor_sync(mask, amax, 1));
   const Scale s = block_scale<NV>(amax);
+  float v[16];
+  if (p.unit) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = in_code_units<NV>(v[i], s);
+    for (int i = 0; i < 16; ++i) v[i] = in_code_units<NV>(value_of<T>(w, i), s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = in_code_units<NV>(value_of<T>(w, i) * p.multiplier, s);
+  }
   uint2 codes;
   codes.x = pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
   codes.y = pack8(v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]);
   if (s.byte == Format<NV>::NAN_SCALE) codes = make_uint2(0u, 0u);
-  if (row < p.rows && k0 / 2 < p.code_bytes)
-    *reinterpret_cast<uint2*>(p.codes + row * p.pitch + k0 / 2) = codes;
-  const uint32_t in_word = chunk % PER_WORD;
-  uint32_t word = (row < p.rows ? s.byte : 0u) << (8 * (NV ? in_word : in_word / 2));
-#pragma unroll
-  for (int d = PER_WORD / 4; d < PER_WORD; d *= 2) word |= __shfl_xor_sync(mask, word, d);
-  if (in_word == 0) *reinterpret_cast<uint32_t*>(p.scales + scale_word(row, chunk / PER_WORD, p.groups)) = word;
+  scale = s.byte;
+  return codes;
 }
 
-// K strided: element k of row i at in[k * ld + i].  A block takes 64 rows x 128 k through shared
-// memory: it is filled along the rows (128 or 256 bytes per k) and read along k, four threads side by
-// side on one row with 32 k each, so that a row's 64 bytes of codes are written together.  The 16
-// extra elements per 32 k put the four threads' words in different banks.
-constexpr int COL_ROWS = 64, COL_K = 128;
+// The four scales of a word, put together among the lanes that hold them; valid in all of them.
+// `in_word` counts the lanes from the word's first one.
+template <bool NV>
+__device__ __forceinline__ uint32_t gather_word(uint32_t byte, uint32_t in_word, uint32_t mask) {
+  constexpr int PER_WORD = NV ? 4 : 8;
+  uint32_t word = byte << (8 * (NV ? in_word : in_word / 2));
+#pragma unroll
+  for (int d = PER_WORD / 4; d < PER_WORD; d *= 2) word |= __shfl_xor_sync(mask, word, d);
+  return word;
+}
+
+// A block's part of the row layout: piece of the row's chunks, first row.
+__device__ __forceinline__ bool row_item(const QuantParams& p, int64_t& row, int64_t& chunk, int rows_per_thread) {
+  const uint32_t in = (threadIdx.x * p.inv_threads) >> 16;  // row of the block; exact for indexes below 256
+  const int64_t piece = static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y;
+  row = static_cast<int64_t>(blockIdx.x) * p.block_rows * rows_per_thread + in;
+  chunk = piece * p.row_threads + (threadIdx.x - in * p.row_threads);
+  return in < p.block_rows;
+}
+
+// Rows with K contiguous.  A thread takes 16 consecutive elements (32 bytes of a 16-bit type in one
+// load) of two rows, both loads before any arithmetic; 16 elements are one e4m3 block or half of an e8m0
+// block.  The lanes that share a 4-byte word of scales are neighbours, so amax and the word are put
+// together with shuffles.  Rows beyond the last up to the next multiple of 128 exist in the scale array
+// only and get zero bytes.
+constexpr int ROWS_PER_THREAD = 2;
+template <typename T, bool NV>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p) {
+  constexpr int PER_WORD = NV ? 4 : 8;  // lanes whose blocks share a word of scales
+  constexpr int WORDS = 4 * sizeof(T);  // of 16 values
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  int64_t row0, chunk;
+  const bool mine = row_item(p, row0, chunk, ROWS_PER_THREAD) && chunk / PER_WORD < p.groups;
+  const uint32_t mask = __ballot_sync(__activemask(), mine);  // whole words: row_threads is a multiple of PER_WORD
+  if (!mine) return;
+  const int64_t k0 = chunk * 16;
+  uint32_t w[ROWS_PER_THREAD][WORDS];
+#pragma unroll
+  for (int r = 0; r < ROWS_PER_THREAD; ++r) {
+    const int64_t row = row0 + r * p.block_rows;
+    const T* src = static_cast<const T*>(p.in) + row * p.ld + k0;
+    if (row < p.rows && k0 + 16 <= p.k && p.vec) {
+#pragma unroll
+      for (int l = 0; l < WORDS / 8; ++l) load32(src + l * (32 / sizeof(T)), *reinterpret_cast<uint32_t(*)[8]>(&w[r][8 * l]));
+    } else {
+      T e[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = (row < p.rows && k0 + i < p.k) ? src[i] : from_float<T>(0.0f);
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[r][i] = reinterpret_cast<const uint32_t*>(e)[i];
+    }
+  }
+  const int64_t rows_padded = (p.rows + 127) & ~static_cast<int64_t>(127);
+#pragma unroll
+  for (int r = 0; r < ROWS_PER_THREAD; ++r) {
+    const int64_t row = row0 + r * p.block_rows;
+    uint32_t byte;
+    const uint2 codes = encode16<T, NV>(w[r], p, mask, byte);
+    if (row < p.rows && k0 / 2 < p.code_bytes) *reinterpret_cast<uint2*>(p.codes + row * p.pitch + k0 / 2) = codes;
+    const uint32_t in_word = static_cast<uint32_t>(chunk) % PER_WORD;
+    const uint32_t word = gather_word<NV>(row < p.rows ? byte : 0u, in_word, mask);
+    if (in_word == 0 && row < rows_padded)
+      *reinterpret_cast<uint32_t*>(p.scales + scale_word(row, chunk / PER_WORD, p.groups)) = word;
+  }
+}
+
+// K strided: element k of row i at in[k * ld + i].  A block takes ROWS rows x 128 k through shared
+// memory: filled along the rows (128 bytes per k), read along k.  A thread takes 16 k of two neighbouring
+// rows (one 32- or 64-bit word of shared memory per k); eight threads side by side hold a row's 128 k, so
+// that its 64 bytes of codes are written together.  The eight extra elements per 16 k put the
+// eight threads' words in different banks.
+constexpr int COL_K = 128;
 template <typename T>
 struct ColTile {
-  static constexpr int PAD = 32 / sizeof(T);  // eight words
-  static constexpr int ELEMS = COL_ROWS * COL_K + 4 * PAD;
-  static __device__ __forceinline__ int at(int k, int row) { return k * COL_ROWS + (k >> 5) * PAD + row; }
+  static constexpr int ROWS = 128 / sizeof(T);
+  static constexpr int THREADS = ROWS * 4;
+  static constexpr int VEC = 16 / sizeof(T);
+  static constexpr int PER_LINE = ROWS / VEC;  // 16-byte pieces of a line
+  static constexpr int PITCH = ROWS;
+  static constexpr int ELEMS = ROWS * COL_K + 8 * 8;
+  static __device__ __forceinline__ int at(int k, int row) { return k * PITCH + (k >> 4) * 8 + row; }
 };
 
 template <typename T, bool NV>
-__global__ void __launch_bounds__(256) quantize_cols_kernel(const QuantParams p) {
-  __shared__ __align__(16) T tile[ColTile<T>::ELEMS];
-  constexpr int VEC = 16 / sizeof(T);
+__global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(const QuantParams p) {
+  using Tile = ColTile<T>;
+  __shared__ __align__(16) T tile[Tile::ELEMS];
+  constexpr int LINES = COL_K * Tile::PER_LINE / Tile::THREADS;  // 16-byte pieces per thread
+  constexpr int VEC = Tile::VEC;
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  const int64_t row_tiles = ((p.rows + 127) / 128) * 2;
-  const int64_t k0 = (blockIdx.x / row_tiles) * COL_K, row0 = (blockIdx.x % row_tiles) * COL_ROWS;
-  const T* const src = static_cast<const T*>(p.in);
-  constexpr int PER_LINE = COL_ROWS / VEC;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * Tile::ROWS;
+  const int64_t k0 = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * COL_K;
+  if (k0 >= p.k) return;
+  const T* const src = static_cast<const T*>(p.in) + k0 * p.ld + row0;
+  const int line = threadIdx.x / Tile::PER_LINE, piece = (threadIdx.x % Tile::PER_LINE) * VEC;
+  constexpr int STEP = Tile::THREADS / Tile::PER_LINE;  // lines per pass
+  uint4 w[LINES];
+  if (p.vec && k0 + COL_K <= p.k && row0 + Tile::ROWS <= p.rows) {
 #pragma unroll
-  for (int l = 0; l < COL_K * PER_LINE / 256; ++l) {
-    const int at = l * 256 + threadIdx.x;
-    const int kk = at / PER_LINE, r = (at % PER_LINE) * VEC;
-    const int64_t gk = k0 + kk, gr = row0 + r;
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (gk < p.k) {
-      if (gr + VEC <= p.rows && p.vec) {
-        w = *reinterpret_cast<const uint4*>(src + gk * p.ld + gr);
-      } else {
-        T* e = reinterpret_cast<T*>(&w);
+    for (int l = 0; l < LINES; ++l)
+      w[l] = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(l * STEP + line) * p.ld + piece);
+  } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (gr + i < p.rows) e[i] = src[gk * p.ld + gr + i];
+    for (int l = 0; l < LINES; ++l) {
+      w[l] = make_uint4(0u, 0u, 0u, 0u);
+      const int kk = l * STEP + line;
+      if (k0 + kk < p.k) {
+        const T* s = src + static_cast<int64_t>(kk) * p.ld + piece;
+        if (row0 + piece + VEC <= p.rows && p.vec) {
+          w[l] = *reinterpret_cast<const uint4*>(s);
+        } else {
+          T* e = reinterpret_cast<T*>(&w[l]);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (row0 + piece + i < p.rows) e[i] = s[i];
+        }
       }
     }
-    *reinterpret_cast<uint4*>(&tile[ColTile<T>::at(kk, r)]) = w;
   }
+#pragma unroll
+  for (int l = 0; l < LINES; ++l) *reinterpret_cast<uint4*>(&tile[Tile::at(l * STEP + line, piece)]) = w[l];
   __syncthreads();
-  const int r = threadIdx.x >> 2, quarter = threadIdx.x & 3;
-  const int64_t row = row0 + r;
-  float v[32];
+  const uint32_t c = threadIdx.x & 7u;                 // chunk of 16 k
+  const int pair = static_cast<int>(threadIdx.x >> 3) * 2;  // first of the two rows
+  uint32_t v[2][4 * sizeof(T)];
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = to_float<T>(tile[ColTile<T>::at(quarter * 32 + i, r)]) * p.multiplier;
-  uint32_t bytes = 0;  // this thread's one or two scales
-  constexpr int BLOCK = Format<NV>::BLOCK;
-  uint32_t codes[4];
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = *reinterpret_cast<const uint32_t*>(&tile[Tile::at(c * 16 + 2 * i, pair)]);
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(&tile[Tile::at(c * 16 + 2 * i + 1, pair)]);
+      v[0][i] = __byte_perm(a, b, 0x5410);
+      v[1][i] = __byte_perm(a, b, 0x7632);
+    }
+  } else {
 #pragma unroll
-  for (int b = 0; b < 32 / BLOCK; ++b) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < BLOCK; ++i) amax = amax_nan(amax, v[b * BLOCK + i]);
-    const Scale s = block_scale<NV>(amax);
-    bytes |= s.byte << (8 * b);
-#pragma unroll
-    for (int i = 0; i < BLOCK / 8; ++i) {
-      float* x = &v[b * BLOCK + i * 8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = in_code_units<NV>(x[j], s);
-      const uint32_t c = pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
-      codes[b * (BLOCK / 8) + i] = s.byte == Format<NV>::NAN_SCALE ? 0u : c;
+    for (int i = 0; i < 16; ++i) {
+      const uint2 a = *reinterpret_cast<const uint2*>(&tile[Tile::at(c * 16 + i, pair)]);
+      v[0][i] = a.x;
+      v[1][i] = a.y;
     }
   }
-  const int64_t at = (k0 + quarter * 32) / 2;
-  if (row < p.rows && at < p.code_bytes)
-    *reinterpret_cast<uint4*>(p.codes + row * p.pitch + at) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-  if (row >= p.rows) bytes = 0;
-  if constexpr (!NV) {
-    uint32_t word = bytes << (8 * quarter);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 1);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
-    if (quarter == 0) *reinterpret_cast<uint32_t*>(p.scales + scale_word(row, k0 / 128, p.groups)) = word;
-  } else {
-    uint32_t word = bytes << (16 * (quarter & 1));
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 1);
-    const int64_t g = k0 / 64 + quarter / 2;
-    if ((quarter & 1) == 0 && g < p.groups) *reinterpret_cast<uint32_t*>(p.scales + scale_word(row, g, p.groups)) = word;
+  const int64_t rows_padded = (p.rows + 127) & ~static_cast<int64_t>(127);
+  const int64_t at = k0 / 2 + c * 8;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int64_t row = row0 + pair + r;
+    uint32_t byte;
+    const uint2 codes = encode16<T, NV>(v[r], p, 0xFFFFFFFFu, byte);
+    if (row < p.rows && at < p.code_bytes) *reinterpret_cast<uint2*>(p.codes + row * p.pitch + at) = codes;
+    constexpr uint32_t PER_WORD = NV ? 4 : 8;
+    const uint32_t word = gather_word<NV>(row < p.rows ? byte : 0u, c % PER_WORD, 0xFFFFFFFFu);
+    const int64_t g = NV ? k0 / 64 + c / 4 : k0 / 128;
+    if (c % PER_WORD == 0 && row < rows_padded && g < p.groups)
+      *reinterpret_cast<uint32_t*>(p.scales + scale_word(row, g, p.groups)) = word;
   }
 }
 
-// code * scale is exact in fp32; the product with the multiplier is rounded once there and once to T.
-template <bool NV>
-__device__ __forceinline__ float scale_of(const QuantParams& p, int64_t row, int64_t block) {
-  return scale_value<NV>(__ldg(p.scales + scale_word(row, block >> 2, p.groups) + (block & 3)));
-}
-
+// Dequantising: code * scale is exact in fp32; the product with the multiplier is rounded once there and
+// once to T.
 template <typename T, bool NV>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(const QuantParams p) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x;
-  if (first + threadIdx.x >= p.items) return;
-  int64_t row;
-  uint32_t chunk;
-  item_coords(p, first, threadIdx.x, row, chunk);
-  const int64_t k0 = static_cast<int64_t>(chunk) * 16;
-  const uint2 codes = *reinterpret_cast<const uint2*>(p.codes + row * p.pitch + k0 / 2);
-  const float s = scale_of<NV>(p, row, k0 / Format<NV>::BLOCK);
-  float v[16];
-  unpack8(codes.x, *reinterpret_cast<float(*)[8]>(&v[0]));
-  unpack8(codes.y, *reinterpret_cast<float(*)[8]>(&v[8]));
+  int64_t row0, chunk;
+  if (!row_item(p, row0, chunk, ROWS_PER_THREAD) || chunk * 16 >= p.k) return;
+  const int64_t k0 = chunk * 16;
+  uint2 codes[ROWS_PER_THREAD];
+  uint32_t bytes[ROWS_PER_THREAD];
+  constexpr int BLOCK = Format<NV>::BLOCK;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = v[i] * s * p.multiplier;
-  T* dst = static_cast<T*>(p.out) + row * p.ld + k0;
-  if (k0 + 16 <= p.k && p.vec) {
-    constexpr int STORES = sizeof(T) / 2;
-#pragma unroll
-    for (int l = 0; l < STORES; ++l) {
-      uint32_t w[8];
-      T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-      for (int i = 0; i < 16 / STORES; ++i) e[i] = from_float<T>(v[l * (16 / STORES) + i]);
-      store32(dst + l * (16 / STORES), w);
+  for (int r = 0; r < ROWS_PER_THREAD; ++r) {
+    const int64_t row = row0 + r * p.block_rows;
+    if (row < p.rows) {
+      codes[r] = *reinterpret_cast<const uint2*>(p.codes + row * p.pitch + k0 / 2);
+      const int64_t block = k0 / BLOCK;
+      bytes[r] = __ldg(p.scales + scale_word(row, block >> 2, p.groups) + (block & 3));
     }
-  } else {
+  }
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (k0 + i < p.k) dst[i] = from_float<T>(v[i]);
+  for (int r = 0; r < ROWS_PER_THREAD; ++r) {
+    const int64_t row = row0 + r * p.block_rows;
+    if (row >= p.rows) break;
+    const float s = scale_value<NV>(bytes[r]);
+    float v[16];
+    unpack8(codes[r].x, *reinterpret_cast<float(*)[8]>(&v[0]));
+    unpack8(codes[r].y, *reinterpret_cast<float(*)[8]>(&v[8]));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = v[i] * s * p.multiplier;
+    T* dst = static_cast<T*>(p.out) + row * p.ld + k0;
+    if (k0 + 16 <= p.k && p.vec) {
+      constexpr int STORES = sizeof(T) / 2;
+#pragma unroll
+      for (int l = 0; l < STORES; ++l) {
+        uint32_t w[8];
+        T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+        for (int i = 0; i < 16 / STORES; ++i) e[i] = from_float<T>(v[l * (16 / STORES) + i]);
+        store32(dst + l * (16 / STORES), w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + i < p.k) dst[i] = from_float<T>(v[i]);
+    }
   }
 }
 
+// The inverse of quantize_cols_kernel, with the same tile and the same division of work.
 template <typename T, bool NV>
-__global__ void __launch_bounds__(256) dequantize_cols_kernel(const QuantParams p) {
-  __shared__ __align__(16) T tile[ColTile<T>::ELEMS];
-  constexpr int VEC = 16 / sizeof(T);
+__global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(const QuantParams p) {
+  using Tile = ColTile<T>;
+  __shared__ __align__(16) T tile[Tile::ELEMS];
+  constexpr int VEC = Tile::VEC;
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  const int64_t row_tiles = (p.rows + COL_ROWS - 1) / COL_ROWS;
-  const int64_t k0 = (blockIdx.x / row_tiles) * COL_K, row0 = (blockIdx.x % row_tiles) * COL_ROWS;
-  const int r = threadIdx.x >> 2, quarter = threadIdx.x & 3;
-  const int64_t row = row0 + r, kq = k0 + quarter * 32;
-  if (row < p.rows && kq < p.k) {
-    const uint4 c = *reinterpret_cast<const uint4*>(p.codes + row * p.pitch + kq / 2);
-    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-    constexpr int BLOCK = Format<NV>::BLOCK;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * Tile::ROWS;
+  const int64_t k0 = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * COL_K;
+  if (k0 >= p.k) return;
+  const int c = static_cast<int>(threadIdx.x & 7u), pair = static_cast<int>(threadIdx.x >> 3) * 2;
+  const int64_t kc = k0 + c * 16;
+  uint2 codes[2] = {};
+  uint32_t bytes[2] = {};
+  constexpr int BLOCK = Format<NV>::BLOCK;
 #pragma unroll
-    for (int b = 0; b < 32 / BLOCK; ++b) {
-      const int64_t block = kq / BLOCK + b;
-      const float s = block * BLOCK < p.k ? scale_of<NV>(p, row, block) : 0.0f;
-#pragma unroll
-      for (int i = 0; i < BLOCK / 8; ++i) {
-        float v[8];
-        unpack8(words[b * (BLOCK / 8) + i], v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          tile[ColTile<T>::at(quarter * 32 + b * BLOCK + i * 8 + j, r)] = from_float<T>(v[j] * s * p.multiplier);
-      }
+  for (int r = 0; r < 2; ++r) {
+    const int64_t row = row0 + pair + r;
+    if (row < p.rows && kc < p.k) {
+      codes[r] = *reinterpret_cast<const uint2*>(p.codes + row * p.pitch + kc / 2);
+      const int64_t block = kc / BLOCK;
+      bytes[r] = __ldg(p.scales + scale_word(row, block >> 2, p.groups) + (block & 3));
     }
   }
-  __syncthreads();
-  T* const dst = static_cast<T*>(p.out);
-  constexpr int PER_LINE = COL_ROWS / VEC;
+  float v[2][16];
 #pragma unroll
-  for (int l = 0; l < COL_K * PER_LINE / 256; ++l) {
-    const int at = l * 256 + threadIdx.x;
-    const int kk = at / PER_LINE, rr = (at % PER_LINE) * VEC;
-    const int64_t gk = k0 + kk, gr = row0 + rr;
-    if (gk >= p.k) break;
-    const T* e = &tile[ColTile<T>::at(kk, rr)];
-    if (gr + VEC <= p.rows && p.vec) {
-      *reinterpret_cast<uint4*>(dst + gk * p.ld + gr) = *reinterpret_cast<const uint4*>(e);
+  for (int r = 0; r < 2; ++r) {
+    const float s = scale_value<NV>(bytes[r]);
+    unpack8(codes[r].x, *reinterpret_cast<float(*)[8]>(&v[r][0]));
+    unpack8(codes[r].y, *reinterpret_cast<float(*)[8]>(&v[r][8]));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[r][i] = v[r][i] * s * p.multiplier;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    T both[2] = {from_float<T>(v[0][i]), from_float<T>(v[1][i])};
+    T* const to = &tile[Tile::at(c * 16 + i, pair)];
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(both);
+    else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(both);
+  }
+  __syncthreads();
+  T* const dst = static_cast<T*>(p.out) + k0 * p.ld + row0;
+  const int line = threadIdx.x / Tile::PER_LINE, piece = (threadIdx.x % Tile::PER_LINE) * VEC;
+  constexpr int STEP = Tile::THREADS / Tile::PER_LINE;
+#pragma unroll
+  for (int l = 0; l < COL_K / STEP; ++l) {
+    const int kk = l * STEP + line;
+    if (k0 + kk >= p.k) break;
+    const T* e = &tile[Tile::at(kk, piece)];
+    T* d = dst + static_cast<int64_t>(kk) * p.ld + piece;
+    if (row0 + piece + VEC <= p.rows && p.vec) {
+      *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(e);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (gr + i < p.rows) dst[gk * p.ld + gr + i] = e[i];
+        if (row0 + piece + i < p.rows) d[i] = e[i];
     }
   }
 }

@@ -16,7 +16,7 @@ struct QuantParams;
 }
 
 struct MxEntry {
-  // cluster: CTAs per cluster (2 for a pair tile, the split of a swapped tile otherwise)
+  // cluster: CTAs per cluster (CTAs of a tile x CTAs or pairs that share its K range)
   cudaError_t (*launch)(const MxMaps&, const MxParams&, int grid, int cluster, cudaStream_t);
   cudaError_t (*attr)();
   int stages, smem_bytes;
@@ -27,8 +27,8 @@ MxEntry mx_kernels_fp4(int config, bool gated);
 MxEntry mx_kernels_nvfp4(int config, bool gated);
 
 // type: GZ_DT_F16, GZ_DT_BF16 or GZ_DT_F32; cols: the values have K strided.
-cudaError_t mx_launch_quantize(int type, bool nv, bool cols, const mx::QuantParams& p, int64_t blocks, cudaStream_t stream);
-cudaError_t mx_launch_dequantize(int type, bool nv, bool cols, const mx::QuantParams& p, int64_t blocks, cudaStream_t stream);
+cudaError_t mx_launch_quantize(int type, bool nv, bool cols, const mx::QuantParams& p, cudaStream_t stream);
+cudaError_t mx_launch_dequantize(int type, bool nv, bool cols, const mx::QuantParams& p, cudaStream_t stream);
 
 }  // namespace gz
 #endif

@@ -47,10 +47,9 @@ def test_sizes():
     (dict(out_type=gz.DT_S8), api.GZ_ERR_UNSUPPORTED), (dict(out_type=FP4), api.GZ_ERR_UNSUPPORTED),
     (dict(out_type=FP4, gated=True), api.GZ_OK), (dict(out_type=NV, gated=True), api.GZ_OK),
     (dict(config=6), api.GZ_ERR_INVALID_ARG), (dict(split=3), api.GZ_ERR_INVALID_ARG),
-    (dict(config=gz.MX_CFG_PAIR, split=2), api.GZ_ERR_UNSUPPORTED),
+    (dict(config=gz.MX_CFG_PAIR, split=8), api.GZ_ERR_UNSUPPORTED), (dict(config=gz.MX_CFG_SINGLE, split=8, gated=True), api.GZ_ERR_UNSUPPORTED),
     (dict(config=gz.MX_CFG_SWAP_M16, m=17), api.GZ_ERR_UNSUPPORTED),
     (dict(config=gz.MX_CFG_SWAP_M16, m=4, n=128, split=8), api.GZ_ERR_UNSUPPORTED),   # one K block
-    (dict(config=gz.MX_CFG_SWAP_M16, m=4, n=128 * 100, k=4096, split=2), api.GZ_ERR_UNSUPPORTED),  # two waves
     (dict(flags=1), api.GZ_ERR_INVALID_ARG),
     (dict(pitch_a=8), api.GZ_ERR_INVALID_ARG), (dict(pitch_a=136), api.GZ_ERR_MISALIGNED),
     (dict(ldd=100), api.GZ_ERR_INVALID_ARG), (dict(ldc=255), api.GZ_ERR_INVALID_ARG),
@@ -88,8 +87,8 @@ def test_struct_size_and_null_arguments():
     (dict(multiplier=float("nan")), api.GZ_ERR_INVALID_ARG), (dict(multiplier=float("inf")), api.GZ_ERR_INVALID_ARG),
     (dict(device=-1), api.GZ_ERR_INVALID_ARG), (dict(src=4097), api.GZ_ERR_MISALIGNED),
     (dict(codes=4104), api.GZ_ERR_MISALIGNED), (dict(scales=4104), api.GZ_ERR_MISALIGNED),
-    (dict(rows=2 ** 31), api.GZ_ERR_TOO_LARGE), (dict(rows=2 ** 30, k=2 ** 30, ld=2 ** 30), api.GZ_ERR_TOO_LARGE),
-    (dict(rows=2 ** 30, ld=2 ** 62), api.GZ_ERR_TOO_LARGE),
+    (dict(rows=2 ** 31), api.GZ_ERR_TOO_LARGE), (dict(rows=2 ** 30, k=2 ** 30, ld=2 ** 31), api.GZ_ERR_TOO_LARGE),
+    (dict(rows=2 ** 30, ld=2 ** 60), api.GZ_ERR_TOO_LARGE),
 ])
 def test_quantize_checks(kw, expect):
     """Every refusal comes before the device is touched (the addresses are never used)."""
@@ -119,9 +118,13 @@ def test_without_a_gpu_there_is_no_fallback():
 def test_every_choice_can_be_launched(m, n, k, gated):
     for fmt in FORMATS:
         st, i = gz.mx_validate(gz.MxDesc.make(fmt, gz.DT_BF16, m, n, k, gated))
-        assert st == api.GZ_OK and i.smem_bytes <= 232448 and i.stages >= 4
-        assert 1 <= i.grid <= 148 and i.grid % (2 if i.config == gz.MX_CFG_PAIR else i.split) == 0
-        assert i.split == 1 or (i.grid == i.tiles * i.split and i.split <= -(-k // 256))
+        assert st == api.GZ_OK and i.smem_bytes <= 232448 and i.stages >= 2
+        ctas = 2 if i.config == gz.MX_CFG_PAIR else 1
+        assert i.grid >= 1 and i.grid % (ctas * i.split) == 0 and ctas * i.split <= 8 and i.split <= -(-k // 256)
+        if i.split > 1 or i.config >= gz.MX_CFG_SWAP_M16:
+            assert i.grid == i.tiles * i.split * ctas
+        else:
+            assert i.grid <= 148
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -268,9 +271,9 @@ def _mx(rows, k, fmt, seed, integers=False):
     return q, orc.decode(codes, scales, fmt)
 
 
-CONFIGS = [gz.MX_CFG_PAIR, gz.MX_CFG_SWAP_M16, gz.MX_CFG_SWAP_M32, gz.MX_CFG_SWAP_M64, gz.MX_CFG_SWAP_M128]
+CONFIGS = [gz.MX_CFG_PAIR, gz.MX_CFG_SINGLE, gz.MX_CFG_SWAP_M16, gz.MX_CFG_SWAP_M32, gz.MX_CFG_SWAP_M64]
 ROWS = {gz.MX_CFG_PAIR: [1, 200, 300, 520], gz.MX_CFG_SWAP_M16: [1, 13, 16], gz.MX_CFG_SWAP_M32: [1, 17, 32],
-        gz.MX_CFG_SWAP_M64: [33, 64], gz.MX_CFG_SWAP_M128: [1, 100, 128, 257]}
+        gz.MX_CFG_SWAP_M64: [33, 64], gz.MX_CFG_SINGLE: [1, 100, 128, 257]}
 GUARD = 77.0
 
 
@@ -304,8 +307,9 @@ def test_product_of_integers_is_exact(fmt, config):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_SWAP_M16, 5, 2), (gz.MX_CFG_SWAP_M16, 16, 4), (gz.MX_CFG_SWAP_M16, 1, 8),
-                                            (gz.MX_CFG_SWAP_M32, 21, 8), (gz.MX_CFG_SWAP_M64, 50, 4), (gz.MX_CFG_SWAP_M128, 128, 8),
-                                            (gz.MX_CFG_SWAP_M128, 200, 2)])
+                                            (gz.MX_CFG_SWAP_M32, 21, 8), (gz.MX_CFG_SWAP_M64, 50, 4), (gz.MX_CFG_SINGLE, 128, 4),
+                                            (gz.MX_CFG_SINGLE, 200, 2), (gz.MX_CFG_PAIR, 300, 2),
+                                            (gz.MX_CFG_PAIR, 100, 4)])
 def test_shared_k_ranges(fmt, config, m, split):
     for n, k in [(130, 256 * split), (256, 256 * split + 900), (300, 4096)]:
         a, av = _mx(m, k, fmt, 1, True)
@@ -331,7 +335,7 @@ def _tolerance(want, s, k, dtype):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("config,m", [(gz.MX_CFG_PAIR, 300), (gz.MX_CFG_SWAP_M16, 9), (gz.MX_CFG_SWAP_M128, 130), (gz.MX_CFG_AUTO, 70)])
+@pytest.mark.parametrize("config,m", [(gz.MX_CFG_PAIR, 300), (gz.MX_CFG_SWAP_M16, 9), (gz.MX_CFG_SINGLE, 130), (gz.MX_CFG_AUTO, 70)])
 def test_product_epilogue_terms(fmt, dtype, config, m):
     """alpha, beta (C apart from D and in place), bias, row and column scales; rows of D that TMA can and cannot store."""
     for n, k, ldd in [(264, 700, 264), (301, 1025, 303)]:
@@ -542,7 +546,7 @@ def test_python_refusals():
 
 
 @gpu
-@pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_PAIR, 300, 1), (gz.MX_CFG_SWAP_M16, 4, 4), (gz.MX_CFG_SWAP_M128, 200, 1)])
+@pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_PAIR, 300, 1), (gz.MX_CFG_SWAP_M16, 4, 4), (gz.MX_CFG_SINGLE, 200, 1), (gz.MX_CFG_PAIR, 300, 2)])
 def test_withheld_signal_times_out_and_context_survives(config, m, split):
     n, k = 300, 2048
     a, av = _mx(m, k, FP4, 1, True)
