@@ -19,6 +19,7 @@ from .api import (  # noqa: F401
 )
 from .microscale import (  # noqa: F401
     MX_FP4, MX_NVFP4, MX_CFG_AUTO, MX_CFG_PAIR, MX_CFG_SINGLE, MX_CFG_SWAP_M16, MX_CFG_SWAP_M32, MX_CFG_SWAP_M64,
+    MX_CFG_PAIR_N128, MX_CFG_SINGLE_N128,
     MxDesc, MxGated, MxGemm, MxMatrix, MxPlanInfo, linear_scales, mx_dequantize, mx_quantize, mx_validate, tile_scales,
 )
 

@@ -65,13 +65,15 @@ gz_status mx_quant_params(gz::mx::QuantParams* p, const void* values, int type, 
 
 struct MxShape {
   int config, bn, ctas;
-  bool swap() const { return bn < 256; }
+  bool swap() const { return bn <= 64; }
 };
 const MxShape kMxShapes[] = {{GZ_MX_CFG_PAIR, 256, 2},
                              {GZ_MX_CFG_SINGLE, 256, 1},
                              {GZ_MX_CFG_SWAP_M16, 16, 1},
                              {GZ_MX_CFG_SWAP_M32, 32, 1},
-                             {GZ_MX_CFG_SWAP_M64, 64, 1}};
+                             {GZ_MX_CFG_SWAP_M64, 64, 1},
+                             {GZ_MX_CFG_PAIR_N128, 128, 2},
+                             {GZ_MX_CFG_SINGLE_N128, 128, 1}};
 const MxShape* mx_shape_of(int config) {
   for (const auto& s : kMxShapes)
     if (s.config == config) return &s;
@@ -114,22 +116,29 @@ gz_status mx_normalise(const gz_mx_desc* desc, MxProblem* pr) {
   return GZ_OK;
 }
 
-bool mx_shape_fits(const MxProblem& pr, const MxShape& s) { return !s.swap() || pr.d.m <= s.bn; }
-
-int64_t mx_tiles(const MxProblem& pr, const MxShape& s) {
-  if (!s.swap()) return cdiv(pr.d.m, 128 * s.ctas) * cdiv(pr.d.n, pr.d.gated ? 128 : 256);
-  return cdiv(pr.d.n, 128);
+bool mx_shape_fits(const MxProblem& pr, const MxShape& s) {
+  if (s.swap()) return pr.d.m <= s.bn;
+  return s.bn == 256 || !pr.d.gated;
 }
 
-// The largest cluster is eight CTAs, and a row tile has four (gated) or eight slices of 32 columns to
-// deal to the parts.
-int mx_max_split(const MxProblem& pr, const MxShape& s) { return (s.ctas == 2 || (!s.swap() && pr.d.gated)) ? 4 : 8; }
+// Output columns of a tile.
+int mx_tile_n(const MxProblem& pr, const MxShape& s) { return s.swap() ? 128 : pr.d.gated ? s.bn / 2 : s.bn; }
+
+int64_t mx_tiles(const MxProblem& pr, const MxShape& s) {
+  return (s.swap() ? 1 : cdiv(pr.d.m, 128 * s.ctas)) * cdiv(pr.d.n, mx_tile_n(pr, s));
+}
+
+// The largest cluster is eight CTAs, and a row tile has a slice for every 32 columns to deal to the parts.
+int mx_max_split(const MxProblem& pr, const MxShape& s) {
+  const int slices = s.swap() ? 8 : mx_tile_n(pr, s) / 32, ctas = 8 / s.ctas;
+  return slices < ctas ? slices : ctas;
+}
 
 // CTAs that can be resident at the same time in clusters of `cluster`.  A cluster lies within one GPC;
-// 148 SMs in GPCs of 16 to 20 hold 16 clusters of eight or 33 of four one-per-SM CTAs.  Swapped tiles have
-// two CTAs per SM.
+// 148 SMs in GPCs of 16 to 20 hold 14 clusters of eight or 32 of four one-per-SM CTAs on every part seen.  Swapped tiles
+// have two CTAs per SM.
 int64_t mx_resident(const MxShape& s, int cluster, int sm_count) {
-  const int64_t sms = cluster >= 8 ? sm_count * 128 / 148 : cluster == 4 ? sm_count * 132 / 148 : sm_count;
+  const int64_t sms = cluster >= 8 ? sm_count * 112 / 148 : cluster == 4 ? sm_count * 128 / 148 : sm_count;
   return s.swap() ? 2 * sms : sms;
 }
 
@@ -138,19 +147,19 @@ double mx_cost(const MxProblem& pr, const MxShape& s, int split, int sm_count) {
   const int64_t tiles = mx_tiles(pr, s), k_blocks = cdiv(pr.d.k, 256);
   const bool nv = pr.d.format == GZ_MX_NVFP4;
   const double mb = (s.swap() && pr.d.gated) ? 2.0 : 1.0;
-  const double bytes = (128.0 * mb + double(s.bn) / s.ctas) * 128.0 + 512.0 * (nv ? 4 : 2) * (mb + (s.swap() ? 1 : 2));
+  const double bytes = (128.0 * mb + double(s.bn) / s.ctas) * 128.0 + 512.0 * (nv ? 4 : 2) * (mb + (s.bn > 128 ? 2 : 1));
   const int64_t slots = mx_resident(s, s.ctas * split, sm_count) / (s.ctas * split);  // clusters
   if (slots <= 0) return 1e30;
   const double waves = double(cdiv(tiles, slots));
   const double blocks = double(cdiv(k_blocks, split));
   // clocks per K block: the MMAs; the fill from L2 (and, for all CTAs together, from HBM)
-  const double mma = s.swap() ? 200.0 * mb : 512.0;
+  const double mma = s.swap() ? 200.0 * mb : s.bn == 256 ? 512.0 : s.ctas == 2 ? 300.0 : 330.0;
   const double active = double(tiles * s.ctas * split < slots * s.ctas * split ? tiles * s.ctas * split : slots * s.ctas * split);
   const double per_sm = s.swap() && active > sm_count ? 2.0 : 1.0;
   double per_block = bytes / 60.0 * per_sm;
   if (mma > per_block) per_block = mma;
   if (s.swap() && bytes * active / 3400.0 > per_block) per_block = bytes * active / 3400.0;
-  const double finish = s.swap() ? 600.0 + 12.0 * double(pr.d.m) * mb / split : 3000.0 + (split > 1 ? 2500.0 : 0.0);
+  const double finish = s.swap() ? 600.0 + 12.0 * double(pr.d.m) * mb / split : 12.0 * s.bn + (split > 1 ? 30.0 * s.bn : 0.0);
   const double fixed = 4000.0 + (s.ctas == 2 ? 1500.0 : 0.0) + (split > 1 ? 1500.0 : 0.0);
   if (s.swap()) return waves * (blocks * per_block + finish) + fixed;
   return waves * (blocks * per_block + 300.0) + finish + fixed;
@@ -211,7 +220,7 @@ gz_status mx_resolve(const MxProblem& pr, int sm_count, gz_mx_plan_info* info) {
   info->config = config;
   info->split = split;
   info->tile_m = s.swap() ? s.bn : 128 * s.ctas;
-  info->tile_n = s.swap() || pr.d.gated ? 128 : 256;
+  info->tile_n = mx_tile_n(pr, s);
   info->tile_k = 256;
   info->stages = e.stages;
   info->smem_bytes = e.smem_bytes;
@@ -281,7 +290,8 @@ gz_status mx_launch(gz_mx_plan* pl, gz::MxParams* p, const void* a, const void* 
   bool ok;
   if (!s.swap())
     ok = mx_encode_operand(pl, &maps.wide, &maps.wide_scales, a, a_scales, d.m, d.pitch_a, 128) &&
-         mx_encode_operand(pl, &maps.narrow, &maps.narrow_scales, b, b_scales, d.n, d.pitch_b, 128);
+         mx_encode_operand(pl, &maps.narrow, &maps.narrow_scales, b, b_scales, d.n, d.pitch_b,
+                           s.bn == 256 ? 128u : (uint32_t)(s.bn / s.ctas));
   else
     ok = mx_encode_operand(pl, &maps.wide, &maps.wide_scales, b, b_scales, d.n, d.pitch_b, 128) &&
          mx_encode_operand(pl, &maps.narrow, &maps.narrow_scales, a, a_scales, d.m, d.pitch_a, (uint32_t)s.bn);
@@ -405,6 +415,7 @@ GZ_API gz_status gz_mx_plan_create(gz_mx_plan** out, const gz_mx_desc* desc) {
   p.n = (uint32_t)d.n;
   p.k_blocks = (uint32_t)cdiv(d.k, 256);
   p.split = (uint32_t)info.split;
+  p.prefetch = 2;  // 0 / 2 / 8 blocks at 1 x 14336 x 4096, e4m3 blocks, in a chain: 9.8 / 9.6 / 10.4 us
   // e2m1 operands, N, scale type, M
   p.idesc = (1u << 7) | (1u << 10) | ((uint32_t)(s.bn >> 3) << 17) | ((d.format == GZ_MX_FP4 ? 1u : 0u) << 23) |
             ((uint32_t)(8 * s.ctas) << 24);

@@ -12,8 +12,8 @@
 // in tensor memory need no barrier of their own.
 //
 // Two tile families:
-//   row tiles  256 x 256 on a CTA pair (cta_group::2) or 128 x 256 on one CTA: A's rows on the 128-lane
-//              side.  In a pair each CTA loads its own 128 rows of A and its own 128 rows of B, and the
+//   row tiles  256 x 256 or 256 x 128 on a CTA pair (cta_group::2), 128 x 256 or 128 x 128 on one CTA: A's
+//              rows on the 128-lane side.  In a pair each CTA loads its own 128 rows of A and its own 128 rows of B, and the
 //              scales of all 256 rows of B.  The gated product takes 128 rows of the gate and 128 of the
 //              up projection as its 256 (in a pair CTA 0 loads the gate's, CTA 1 the up projection's):
 //              one MMA computes both halves and no operand is loaded twice.  Two fp32 accumulators of
@@ -27,9 +27,11 @@
 //              is the transpose of the output; it goes through shared memory, after which a warp takes
 //              one output row at a time, a lane four neighbouring columns.
 // Where tiles are fewer than SMs, the CTAs (pairs) of a cluster share a tile's K range.  Their partial
-// sums meet in shared memory, in the ring that the main loop no longer needs; each CTA adds and
-// finishes a share of the tile over distributed shared memory, in rank order, so there is no
-// workspace, nothing to clear and one order of summation.
+// sums meet in shared memory; each CTA adds and finishes a share of the tile, in rank order, so there
+// is no workspace, nothing to clear and one order of summation.  The partial sums lie in the ring that
+// the main loop no longer needs, and the CTA that finishes a share fetches it from its peers 16 bytes a
+// lane.  (Storing each row into the CTA that finishes it instead saves a barrier but measured 0.3 us
+// slower at 16 rows and 2.4 us at 64: remote stores of a word per lane are slow.)
 #ifndef GZ_MX_GEMM_CUH
 #define GZ_MX_GEMM_CUH
 
@@ -53,6 +55,7 @@ struct MxParams {
   uint32_t m, n;  // rows and columns of the output
   uint32_t k_blocks;
   uint32_t split;  // CTAs or CTA pairs (one cluster) that share a tile's K range
+  uint32_t prefetch;  // swapped tiles: K blocks brought into L2 ahead of the launch's dependencies (at most 32)
   uint32_t idesc;
   uint32_t out_type;
   uint32_t out_tma, c_vec_ok;
@@ -76,10 +79,10 @@ template <bool NV_, int BN_, int CTAS_, bool GATED_>
 struct MxCfg {
   static constexpr bool NV = NV_, GATED = GATED_;
   static constexpr int BN = BN_, CTAS = CTAS_;
-  static constexpr bool SWAP = BN < 256;
+  static constexpr bool SWAP = BN <= 64;
   static constexpr int MB = (GATED && SWAP) ? 2 : 1;  // 128-row blocks on the wide side per CTA
   static constexpr int TILES_K = NV ? 4 : 2;          // scale tiles per stage and 128 rows
-  static constexpr int NRB = SWAP ? 1 : 2;            // scale row groups of the narrow side
+  static constexpr int NRB = BN > 128 ? 2 : 1;        // scale row groups of the narrow side
   static constexpr int W_BYTES = MB * 128 * 128;
   static constexpr int N_BYTES = (BN / CTAS) * 128;
   static constexpr int WS_BYTES = MB * TILES_K * 512;
@@ -89,20 +92,22 @@ struct MxCfg {
   static constexpr int STAGING_BYTES = SWAP ? 0 : EPI_WARPS * 4096;
   static constexpr int BAR_BYTES = 512;
   // 227 KB per block; two blocks per SM share 228 KB of which each costs 1 KB more than it asks for
-  static constexpr int SMEM_LIMIT = SWAP ? 115712 : 232448;
+  static constexpr int PER_SM = SWAP ? 2 : 1;
+  static constexpr int SMEM_LIMIT = PER_SM == 2 ? 115712 : 232448;
   static constexpr int STAGES = (SMEM_LIMIT - 1024 - STAGING_BYTES - BAR_BYTES) / STAGE_BYTES;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int SMEM_BYTES = 1024 + RING_BYTES + STAGING_BYTES + BAR_BYTES;
   static constexpr int THREADS = 96 + 32 * EPI_WARPS;
   // Tensor memory: accumulators, then four 16-column scale slots.  (Swapped tiles: at most half of it, so
   // that a second block's allocation never has to wait for the first block.)
-  static constexpr int ACC_COLS = SWAP ? MB * BN : 448;
+  static constexpr int ACC_STRIDE = BN == 256 ? 192 : BN;  // row tiles: from one accumulator to the next
+  static constexpr int ACC_COLS = SWAP ? MB * BN : ACC_STRIDE + BN;
   static constexpr int SLOT_COLS = 16;
   static constexpr int TMEM_COLS = ACC_COLS + 64 <= 128 ? 128 : ACC_COLS + 64 <= 256 ? 256 : 512;
   static_assert(ACC_COLS % 16 == 0 && ACC_COLS + 64 <= TMEM_COLS && (!SWAP || TMEM_COLS <= 256), "tensor memory");
-  static_assert(SWAP ? (BN <= 64 && BN % 16 == 0 && CTAS == 1) : BN == 256, "tile shapes");
+  static_assert(SWAP ? (BN % 16 == 0 && CTAS == 1) : (BN == 256 || (BN == 128 && !GATED)), "tile shapes");
   static_assert(STAGE_BYTES % 1024 == 0 && STAGES >= 2, "ring");
-  static_assert((SWAP ? MB * BN : 256) * 128 * 4 <= RING_BYTES, "partial sums meet in the ring");
+  static_assert(MB * BN * 128 * 4 <= RING_BYTES, "partial sums meet in the ring");
   static_assert(8 * (2 * STAGES + 3) + 16 <= BAR_BYTES, "barriers");
 };
 
@@ -157,9 +162,32 @@ __device__ __forceinline__ float mx_load_c(const MxParams& p, int64_t at) {
   }
 }
 
-// The optional terms on 32 columns of one row (the pair tile).
-__device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], uint32_t row, uint32_t col0,
-                                             uint32_t lane) {
+// 32 columns of one row of C as raw words, where they can be read 16 bytes at a time.  A row tile reads
+// them ahead of the sums they are added to: a lane's row is 64 or 128 bytes at an address of its
+// own, so the loads are all latency.
+__device__ __forceinline__ bool mx_c_vectors(const MxParams& p, uint32_t row, uint32_t col0) {
+  return p.beta != 0.0f && p.c_vec_ok && row < p.m && col0 + 32u <= p.n;
+}
+__device__ __forceinline__ void mx_load_c_words(const MxParams& p, uint32_t row, uint32_t col0, uint32_t (&w)[32]) {
+  if (!mx_c_vectors(p, row, col0)) return;
+  const int64_t at = static_cast<int64_t>(row) * p.ldc + col0;
+  const uint4* c4 = p.out_type == 2u ? reinterpret_cast<const uint4*>(static_cast<const float*>(p.c) + at)
+                                     : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c) + at);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    if (q < 4 || p.out_type == 2u) {
+      const uint4 c = c4[q];
+      w[4 * q] = c.x;
+      w[4 * q + 1] = c.y;
+      w[4 * q + 2] = c.z;
+      w[4 * q + 3] = c.w;
+    }
+  }
+}
+
+// The optional terms on 32 columns of one row (row tiles); w: the words that mx_load_c_words read.
+__device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], const uint32_t (&w)[32], uint32_t row,
+                                             uint32_t col0, uint32_t lane) {
   const bool row_ok = row < p.m;
   const uint32_t ncols = p.n - col0 < 32u ? p.n - col0 : 32u;
   const bool col_ok = lane < ncols;
@@ -174,29 +202,11 @@ __device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], 
     for (int i = 0; i < 32; ++i) f[i] *= __shfl_sync(0xFFFFFFFFu, mine, i);
   }
   if (p.beta != 0.0f && row_ok) {
-    const int64_t at = static_cast<int64_t>(row) * p.ldc + col0;
-    if (ncols == 32u && p.c_vec_ok) {
+    if (mx_c_vectors(p, row, col0)) {
       if (p.out_type == 2u) {
-        const float4* c4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.c) + at);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 c = c4[q];
-          f[4 * q] = fmaf(p.beta, c.x, f[4 * q]);
-          f[4 * q + 1] = fmaf(p.beta, c.y, f[4 * q + 1]);
-          f[4 * q + 2] = fmaf(p.beta, c.z, f[4 * q + 2]);
-          f[4 * q + 3] = fmaf(p.beta, c.w, f[4 * q + 3]);
-        }
+        for (int i = 0; i < 32; ++i) f[i] = fmaf(p.beta, __uint_as_float(w[i]), f[i]);
       } else {
-        const uint4* c4 = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c) + at);
-        uint32_t w[16];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint4 c = c4[q];
-          w[4 * q] = c.x;
-          w[4 * q + 1] = c.y;
-          w[4 * q + 2] = c.z;
-          w[4 * q + 3] = c.w;
-        }
         const bool half_in = p.out_type == 0u;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -206,6 +216,7 @@ __device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], 
         }
       }
     } else {
+      const int64_t at = static_cast<int64_t>(row) * p.ldc + col0;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (static_cast<uint32_t>(i) < ncols) f[i] = fmaf(p.beta, mx_load_c(p, at + i), f[i]);
@@ -265,6 +276,7 @@ __device__ __forceinline__ void mx_store_box(const MxParams& p, const void* tm_d
     __syncwarp();
     const uint32_t rows = p.m - row0 < 32u ? p.m - row0 : 32u;
     const bool ok = lane < p.n - col0;
+#pragma unroll 8
     for (uint32_t r = 0; r < rows; ++r) {
       const int64_t at = static_cast<int64_t>(row0 + r) * p.ldd + col0 + lane;
       if (!ok || !GZ_MX_STORE_OK(p, row0 + r, col0 + lane, 1u, p.m, p.n)) continue;
@@ -320,7 +332,7 @@ __device__ __forceinline__ void mx_store_quantized(const MxParams& p, const floa
 // eight lanes share an e8m0 block and four an e4m3 block.
 template <bool NV>
 __device__ __forceinline__ void mx_store_quantized_row(const MxParams& p, const float (&f)[4], uint32_t row, uint32_t col,
-                                                       uint32_t lane) {
+                                                       uint32_t lane, bool live) {
   constexpr int LANES = mx::Format<NV>::BLOCK / 4;
   float v[4];
   float amax = 0.0f;
@@ -336,11 +348,11 @@ __device__ __forceinline__ void mx_store_quantized_row(const MxParams& p, const 
   for (int i = 0; i < 4; ++i) v[i] = mx::in_code_units<NV>(v[i], s);
   uint32_t codes = mx::pack8(v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f);
   if (s.byte == mx::Format<NV>::NAN_SCALE) codes = 0u;
-  if ((col & ~31u) < p.n && GZ_MX_STORE_OK(p, row, col & ~31u, 1u, p.m, p.n))  // the codes of a row fill up whole 32s
+  if (live && (col & ~31u) < p.n && GZ_MX_STORE_OK(p, row, col & ~31u, 1u, p.m, p.n))  // the codes of a row fill up whole 32s
     *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.d) + static_cast<int64_t>(row) * p.ldd + col / 2) =
         static_cast<uint16_t>(codes);
   const int64_t block = col / mx::Format<NV>::BLOCK;
-  if (lane % LANES == 0u && block < 4 * p.d_groups)
+  if (live && lane % LANES == 0u && block < 4 * p.d_groups)
     p.d_scales[mx::scale_word(row, block >> 2, p.d_groups) + (block & 3)] = static_cast<uint8_t>(s.byte);
 }
 
@@ -353,9 +365,11 @@ __device__ __forceinline__ void mx_load4(const float* v, uint32_t n, float (&f)[
 }  // namespace detail
 
 // Finish one output row of a swapped tile: the warp's lanes hold the sums of four neighbouring columns each.
+// live == false does everything but the stores: the epilogue runs this once while it waits for its
+// accumulator, because code that runs cold runs at the speed instructions can be fetched.
 template <class Cfg>
 __device__ __forceinline__ void mx_finish_row(const MxParams& p, float (&f)[4], const float (&u)[4], uint32_t row,
-                                              uint32_t col, uint32_t lane) {
+                                              uint32_t col, uint32_t lane, bool live) {
   const uint32_t have = col >= p.n ? 0u : p.n - col < 4u ? p.n - col : 4u;  // columns that exist
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] *= p.alpha;
@@ -363,8 +377,8 @@ __device__ __forceinline__ void mx_finish_row(const MxParams& p, float (&f)[4], 
     detail::activate_all(f, p.act);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] *= p.alpha_up * u[i];
-    if (p.out_type == MX_OUT_FP4) return detail::mx_store_quantized_row<false>(p, f, row, col, lane);
-    if (p.out_type == MX_OUT_NVFP4) return detail::mx_store_quantized_row<true>(p, f, row, col, lane);
+    if (p.out_type == MX_OUT_FP4) return detail::mx_store_quantized_row<false>(p, f, row, col, lane, live);
+    if (p.out_type == MX_OUT_NVFP4) return detail::mx_store_quantized_row<true>(p, f, row, col, lane, live);
   }
   if (have == 0u || !GZ_MX_STORE_OK(p, row, col, have, p.m, p.n)) return;
   const bool vec = have == 4u && p.d_vec_ok;
@@ -404,6 +418,7 @@ __device__ __forceinline__ void mx_finish_row(const MxParams& p, float (&f)[4], 
     }
     detail::activate_all(f, p.act);
   }
+  if (!live) return;
   const int64_t at = static_cast<int64_t>(row) * p.ldd + col;
   if (p.out_type == 2u) {
     float* d = static_cast<float*>(p.d) + at;
@@ -441,11 +456,12 @@ __device__ __forceinline__ void mx_clear_scale_row(const MxParams& p, uint32_t t
   }
 }
 
-// 32 columns of one row (lane = row) of a row tile, from the sums to the output.
+// 32 columns of one row (lane = row) of a row tile, from the sums x (gated: and y) to the output.  c holds
+// the words of C for these columns on entry and those for (next_row, next_col0) on return. 
 template <class Cfg>
 __device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* tm_d, uint32_t stg, uint32_t lane,
-                                                const uint32_t (&x)[32], const uint32_t (&y)[32], uint32_t row0,
-                                                uint32_t col0, uint32_t& turn) {
+                                                const uint32_t (&x)[32], const uint32_t (&y)[32], uint32_t (&c)[32],
+                                                uint32_t row0, uint32_t col0, uint32_t next_col0, uint32_t& turn) {
   float f[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) f[i] = p.alpha * __uint_as_float(x[i]);
@@ -462,14 +478,20 @@ __device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* t
     }
     if (row0 >= p.m || col0 >= p.n) return;
   } else {
-    if (row0 >= p.m || col0 >= p.n) return;
-    if (p.epi_flags != 0u || p.beta != 0.0f || p.act != 0u) detail::mx_row_terms(p, f, row0 + lane, col0, lane);
+    if (row0 >= p.m || col0 >= p.n) {
+      detail::mx_load_c_words(p, row0 + lane, next_col0, c);  // the first group of an even tile may lie outside
+      return;
+    }
+    if (p.epi_flags != 0u || p.beta != 0.0f || p.act != 0u) {
+      detail::mx_row_terms(p, f, c, row0 + lane, col0, lane);
+      detail::mx_load_c_words(p, row0 + lane, next_col0, c);
+    }
   }
   detail::mx_store_box(p, tm_d, stg, lane, f, row0, col0, turn);
 }
 
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::THREADS, Cfg::SWAP ? 2 : 1)
+__global__ void __launch_bounds__(Cfg::THREADS, Cfg::PER_SM)
 mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
   constexpr int CTAS = Cfg::CTAS, STAGES = Cfg::STAGES, BN = Cfg::BN, MB = Cfg::MB;
   constexpr bool NV = Cfg::NV, SWAP = Cfg::SWAP, GATED = Cfg::GATED;
@@ -553,6 +575,28 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
     const uint32_t my_bytes = is_narrow ? Cfg::N_BYTES + Cfg::NS_BYTES : Cfg::W_BYTES + Cfg::WS_BYTES;
     uint32_t stage = 0, phase = 0;
     bool ok = true;
+    // A swapped tile's first K blocks are brought into L2 while the kernel before this one finishes.  Nothing
+    // is read yet: whatever that kernel still writes to these lines is written to them in L2.
+    if constexpr (SWAP) {
+      const uint32_t nkb = kb_hi - kb_lo;
+      if (lane < (nkb < p.prefetch ? nkb : p.prefetch) && cluster < p.grid.num_tiles) {
+        const uint32_t at = kb_lo + (lane + cluster * 5u) % nkb;
+        const int32_t kx = static_cast<int32_t>(at * 128u), kt = static_cast<int32_t>(at * Cfg::TILES_K);
+        const int32_t rb = static_cast<int32_t>(cluster);
+        if (is_narrow) {
+          ptx::tma_prefetch_3d(&maps.narrow, kx, 0, 0);
+          ptx::tma_prefetch_3d(&maps.narrow_scales, 0, kt, 0);
+        } else {
+          ptx::tma_prefetch_3d(&maps.wide, kx, rb * 128, 0);
+          ptx::tma_prefetch_3d(&maps.wide_scales, 0, kt, rb);
+          if constexpr (MB == 2) {
+            ptx::tma_prefetch_3d(&maps.up, kx, rb * 128, 0);
+            ptx::tma_prefetch_3d(&maps.up_scales, 0, kt, rb);
+          }
+        }
+      }
+      __syncwarp();
+    }
     ptx::grid_dependency_wait();
     for (uint32_t t = cluster; ok && t < p.grid.num_tiles; t += num_clusters) {
       uint32_t tm, tn;
@@ -590,16 +634,21 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
               load(ws + Cfg::TILES_K * 512u, &maps.up_scales, 0, kt, wide_rb);
             }
           } else if constexpr (!SWAP) {
-            // 256 rows as two groups of 128: rows of B, or the gate's and the up projection's
-            const int32_t rb0 = static_cast<int32_t>(GATED ? tn : tn * 2u), rb1 = GATED ? rb0 : rb0 + 1;
-            const CUtensorMap* const second = GATED ? &maps.up : &maps.narrow;
-            const CUtensorMap* const second_scales = GATED ? &maps.up_scales : &maps.narrow_scales;
             const uint32_t nd = dst + Cfg::W_BYTES;
-            if (CTAS == 1 || rank == 0u) load(nd, &maps.narrow, kx, rb0 * 128, 0);
-            if (CTAS == 1) load(nd + 128u * 128u, second, kx, rb1 * 128, 0);
-            else if (rank == 1u) load(nd, second, kx, rb1 * 128, 0);
-            load(ns, &maps.narrow_scales, 0, kt, rb0);
-            load(ns + Cfg::TILES_K * 512u, second_scales, 0, kt, rb1);
+            if constexpr (BN == 256) {
+              // 256 rows as two groups of 128: rows of B, or the gate's and the up projection's
+              const int32_t rb0 = static_cast<int32_t>(GATED ? tn : tn * 2u), rb1 = GATED ? rb0 : rb0 + 1;
+              const CUtensorMap* const second = GATED ? &maps.up : &maps.narrow;
+              const CUtensorMap* const second_scales = GATED ? &maps.up_scales : &maps.narrow_scales;
+              if (CTAS == 1 || rank == 0u) load(nd, &maps.narrow, kx, rb0 * 128, 0);
+              if (CTAS == 1) load(nd + 128u * 128u, second, kx, rb1 * 128, 0);
+              else if (rank == 1u) load(nd, second, kx, rb1 * 128, 0);
+              load(ns, &maps.narrow_scales, 0, kt, rb0);
+              load(ns + Cfg::TILES_K * 512u, second_scales, 0, kt, rb1);
+            } else {
+              load(nd, &maps.narrow, kx, static_cast<int32_t>(tn * BN + rank * (BN / CTAS)), 0);
+              load(ns, &maps.narrow_scales, 0, kt, static_cast<int32_t>(tn * BN / 128u));
+            }
           } else {
             load(dst + Cfg::W_BYTES, &maps.narrow, kx, 0, 0);
             load(ns, &maps.narrow_scales, 0, kt, 0);
@@ -637,7 +686,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
         ok = __all_sync(0xFFFFFFFFu, detail::wait(acc_empty_bar, (it & 1u) ^ 1u, ab, WAIT_MMA_TMEM_EMPTY, t, 0));
         if (!ok) break;
         ptx::tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + (SWAP ? 0u : (it & 1u) * 192u);
+        const uint32_t d_tmem = tmem_base + (SWAP ? 0u : (it & 1u) * Cfg::ACC_STRIDE);
         for (uint32_t kb = kb_lo; kb < kb_hi; ++kb) {
           ok = __all_sync(0xFFFFFFFFu, detail::wait(full_bar(stage), phase, ab, WAIT_MMA_FULL, t, kb));
           if (!ok) break;
@@ -698,165 +747,186 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
     ptx::grid_dependency_wait();
     const uint32_t quad = warp & 3u;
     const uint32_t lanes = tmem_base + ((quad * 32u) << 16);
-    // Partial (or whole) sums in shared memory: [column of the accumulator][128 lanes].
-    const uint32_t park = base + (quad * 32u + lane) * 4u;
     if constexpr (SWAP) {
-      if (cluster < p.grid.num_tiles && detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0)) {
-        ptx::tc_fence_after_sync();
-#pragma unroll 1
-        for (uint32_t sl = 0; sl * 16u < p.m; ++sl) {
-          uint32_t x[MB][16];
-#pragma unroll
-          for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb) ptx::tmem_ld_32x16(lanes + mb * BN + sl * 16u, x[mb]);
-          ptx::tmem_wait_ld();
-#pragma unroll
-          for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb) {
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(park + (mb * BN + sl * 16u + i) * 512u), "r"(x[mb][i]) : "memory");
-          }
-        }
-        ptx::tc_fence_before_sync();
-      }
-    } else {
-      const uint32_t half = warp >= 7u ? 1u : 0u;
-      const uint32_t stg = staging_base + (half * 4u + quad) * 4096u;
-      const uint32_t release = ptx::mapa(acc_empty_bar, leader);
-      uint32_t turn = 0, it = 0;
-      for (uint32_t t = cluster; t < p.grid.num_tiles; t += num_clusters, ++it) {
-        uint32_t tm, tn;
-        tile_coords(p.grid, t, tm, tn);
-        const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
-        if (!detail::wait(acc_full_bar, it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
-        ptx::tc_fence_after_sync();
-        const uint32_t acc = lanes + (it & 1u) * 192u;
-        if (p.split > 1u) {
-#pragma unroll 1
-          for (uint32_t g = 0; g < 4u; ++g) {
-            const uint32_t off = g * 64u + half * 32u;
-            uint32_t x[32];
-            ptx::tmem_ld_32x32(acc + off, x);
-            ptx::tmem_wait_ld();
-#pragma unroll
-            for (uint32_t i = 0; i < 32; ++i)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(park + (off + i) * 512u), "r"(x[i]) : "memory");
-          }
-          ptx::tc_fence_before_sync();
-          break;  // the cluster's only tile
-        }
-        constexpr uint32_t GROUPS = GATED ? 2u : 4u;  // of 64 columns; this warp's half of each is 32 wide
-#pragma unroll 1
-        for (uint32_t s = 0; s < GROUPS; ++s) {
-          // the group that the next tile's accumulator overlaps comes first
-          const uint32_t g = (it & 1u) ? s : (s + GROUPS - 1u) % GROUPS;
-          const uint32_t off = g * 64u + half * 32u;
-          uint32_t x[32], y[32];
-          ptx::tmem_ld_32x32(acc + off, x);
-          if constexpr (GATED) ptx::tmem_ld_32x32(acc + 128u + off, y);
-          ptx::tmem_wait_ld();
-          if (s == 0) {
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(release);
-          }
-          mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, row0, tn * (GATED ? 128u : 256u) + off, turn);
-        }
-        // one release per tile, made above; the rest of this tile's columns are read before the next
-        // tile's release, which is what the tile after that waits for
-        ptx::tc_fence_before_sync();
-      }
-      if (p.split <= 1u && p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
-    }
-  }
-
-  // -------------------------------------------------------------- sums that met in shared memory
-  if (SWAP || p.split > 1u) {
-    __syncwarp();
-    if (p.split > 1u) {
-      ptx::cluster_arrive_release();
-      ptx::cluster_wait_acquire();
-    } else {
-      __syncthreads();
-    }
-    if (cluster < p.grid.num_tiles && !detail::aborted(ab)) {
+      // The accumulator's columns are output rows, its lanes output columns: [operand][row][128 columns].
+      const uint32_t park = base + (quad * 32u + lane) * 4u;
+      const uint32_t mine = base + lane * 16u;
       uint32_t tm, tn;
       tile_coords(p.grid, cluster, tm, tn);
-      if constexpr (SWAP) {
-        // Output rows part, part + split, ... dealt to the block's warps.
-        const uint32_t mine = base + lane * 16u;
-        const uint32_t col = tm * 128u + lane * 4u;
-        for (uint32_t r = part + p.split * warp; r < p.m; r += p.split * (Cfg::THREADS / 32)) {
-          float f[4] = {}, u[4] = {};
+      const uint32_t col = tm * 128u + lane * 4u;
+      bool live = false;  // the first round is the dry one
+      for (uint32_t r = part + p.split * quad;;) {
+        float f[4] = {}, u[4] = {};
+        if (live) {
+          if (r >= p.m) break;
           if (p.split == 1u) {
             ptx::ld_shared_f32x4(mine + r * 512u, f);
             if constexpr (GATED) ptx::ld_shared_f32x4(mine + (BN + r) * 512u, u);
           } else {
-            for (uint32_t q = 0; q < p.split; q += 2u) {  // two peers' loads in flight
-              const uint32_t a0 = ptx::mapa(mine, q) + r * 512u, a1 = ptx::mapa(mine, q + 1u) + r * 512u;
-              float x0[4], x1[4], y0[4], y1[4];
-              ptx::ld_cluster_f32x4(a0, x0);
-              ptx::ld_cluster_f32x4(a1, x1);
-              if constexpr (GATED) {
-                ptx::ld_cluster_f32x4(a0 + BN * 512u, y0);
-                ptx::ld_cluster_f32x4(a1 + BN * 512u, y1);
+            // up to four peers' loads in flight; the sums are taken in rank order
+            for (uint32_t q = 0; q < p.split; q += 4u) {
+              float x[4][4], y[4][4];
+#pragma unroll
+              for (uint32_t e = 0; e < 4; ++e) {
+                if (q + e < p.split) {
+                  const uint32_t at = ptx::mapa(mine, q + e) + r * 512u;
+                  ptx::ld_cluster_f32x4(at, x[e]);
+                  if constexpr (GATED) ptx::ld_cluster_f32x4(at + BN * 512u, y[e]);
+                }
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                f[i] = (f[i] + x0[i]) + x1[i];
-                if constexpr (GATED) u[i] = (u[i] + y0[i]) + y1[i];
+              for (uint32_t e = 0; e < 4; ++e) {
+                if (q + e < p.split) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    f[i] = q + e == 0u ? x[e][i] : f[i] + x[e][i];
+                    if constexpr (GATED) u[i] = q + e == 0u ? y[e][i] : u[i] + y[e][i];
+                  }
+                }
               }
             }
           }
-          mx_finish_row<Cfg>(p, f, u, r, col, lane);
         }
-        if constexpr (GATED) {
-          if (part == 0u)
-            for (uint32_t r = threadIdx.x; r < 128u; r += Cfg::THREADS) mx_clear_scale_row(p, tm, r);
+        if (r < p.m) mx_finish_row<Cfg>(p, f, u, r, col, lane, live);
+        if (live) {
+          r += p.split * 4u;
+          continue;
         }
-      } else if (warp >= 2u && warp != 6u) {
-        // The tile's 32-column slices are dealt to the parts in order; a slice is finished by the warps of
-        // one half, as without a shared K range.
-        const uint32_t quad = warp & 3u, half = warp >= 7u ? 1u : 0u;
-        const uint32_t stg = staging_base + (half * 4u + quad) * 4096u;
-        const uint32_t mine = base + (quad * 32u + lane) * 4u;
-        const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
-        constexpr uint32_t SLICES = GATED ? 4u : 8u;
-        uint32_t turn = 0;
-        for (uint32_t sl = part * SLICES / p.split; sl < (part + 1u) * SLICES / p.split; ++sl) {
-          if ((sl & 1u) != half) continue;
-          float f[32], u[32];
+        live = true;
+        const bool ok = detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0);
+        if (ok) {
+          ptx::tc_fence_after_sync();
+#pragma unroll 1
+          for (uint32_t sl = 0; sl * 16u < p.m; ++sl) {
+            uint32_t x[MB][16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = u[i] = 0.0f;
-          for (uint32_t q = 0; q < p.split; ++q) {
-            const uint32_t peer = ptx::mapa(mine, CTAS == 2 ? q * 2u + rank : q) + sl * 32u * 512u;
-            float x[32];
+            for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb) ptx::tmem_ld_32x16(lanes + mb * BN + sl * 16u, x[mb]);
+            ptx::tmem_wait_ld();
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) x[i] = ptx::ld_cluster_f32(peer + i * 512u);
+            for (uint32_t mb = 0; mb < static_cast<uint32_t>(MB); ++mb) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] += x[i];
-            if constexpr (GATED) {
-#pragma unroll
-              for (uint32_t i = 0; i < 32; ++i) x[i] = ptx::ld_cluster_f32(peer + (128u + i) * 512u);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) u[i] += x[i];
+              for (uint32_t i = 0; i < 16; ++i)
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(park + (mb * BN + sl * 16u + i) * 512u), "r"(x[mb][i]) : "memory");
             }
           }
-          uint32_t x[32], y[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            x[i] = __float_as_uint(f[i]);
-            y[i] = __float_as_uint(u[i]);
-          }
-          mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, row0, tn * (GATED ? 128u : 256u) + sl * 32u, turn);
+          ptx::tc_fence_before_sync();
         }
-        if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
+        if (p.split > 1u) {
+          __syncwarp();
+          ptx::cluster_arrive_release();
+          ptx::cluster_wait_acquire();
+        } else {
+          ptx::named_barrier_sync(1, 128);
+        }
+        if (!ok || detail::aborted(ab)) break;
       }
+      if constexpr (GATED) {
+        if (part == 0u && !detail::aborted(ab)) mx_clear_scale_row(p, tm, quad * 32u + lane);
+      }
+    } else {
+      const uint32_t half = warp >= 7u ? 1u : 0u;
+      const uint32_t stg = staging_base + (half * 4u + quad) * 4096u;
+      constexpr uint32_t TILE_COLS = GATED ? BN / 2u : BN;  // output columns
+      constexpr uint32_t GROUPS = TILE_COLS / 64u;          // of 64; this warp's half of each is 32 wide
+      uint32_t turn = 0;
+      if (p.split <= 1u) {
+        const uint32_t release = ptx::mapa(acc_empty_bar, leader);
+        uint32_t it = 0;
+        for (uint32_t t = cluster; t < p.grid.num_tiles; t += num_clusters, ++it) {
+          uint32_t tm, tn;
+          tile_coords(p.grid, t, tm, tn);
+          const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
+          const uint32_t tile_col = tn * TILE_COLS + half * 32u;
+          // the group that the next tile's accumulator overlaps comes first
+          auto group_col = [&](uint32_t s) { return tile_col + ((it & 1u) ? s : (s + GROUPS - 1u) % GROUPS) * 64u; };
+          uint32_t c[32];
+          if constexpr (!GATED) detail::mx_load_c_words(p, row0 + lane, group_col(0), c);
+          if (!detail::wait(acc_full_bar, it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
+          ptx::tc_fence_after_sync();
+          const uint32_t acc = lanes + (it & 1u) * Cfg::ACC_STRIDE;
+#pragma unroll 1
+          for (uint32_t s = 0; s < GROUPS; ++s) {
+            const uint32_t col0 = group_col(s), off = col0 - tile_col + half * 32u;
+            uint32_t x[32], y[32];
+            ptx::tmem_ld_32x32(acc + off, x);
+            if constexpr (GATED) ptx::tmem_ld_32x32(acc + BN / 2u + off, y);
+            ptx::tmem_wait_ld();
+            if (s == 0) {
+              ptx::tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive_cluster(release);
+            }
+            mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, c, row0, col0, s + 1u < GROUPS ? group_col(s + 1u) : p.n, turn);
+          }
+          // one release per tile, made above; the rest of this tile's columns are read before the next
+          // tile's release, which is what the tile after that waits for
+          ptx::tc_fence_before_sync();
+        }
+      } else {
+        // The cluster's one tile.  Partial sums lie as [four columns][128 rows][4]: a lane writes or reads 16
+        // bytes, a warp 512 in a row.
+        uint32_t tm, tn;
+        tile_coords(p.grid, cluster, tm, tn);
+        const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
+        const uint32_t mine = base + (quad * 32u + lane) * 16u;
+        const bool ok = detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0);
+        if (ok) {
+          ptx::tc_fence_after_sync();
+#pragma unroll 1
+          for (uint32_t g = 0; g < BN / 64u; ++g) {
+            const uint32_t off = g * 64u + half * 32u;
+            uint32_t x[32];
+            ptx::tmem_ld_32x32(lanes + off, x);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (off / 4u + i) * 2048u), "r"(x[4 * i]),
+                           "r"(x[4 * i + 1]), "r"(x[4 * i + 2]), "r"(x[4 * i + 3])
+                           : "memory");
+          }
+          ptx::tc_fence_before_sync();
+        }
+        __syncwarp();
+        ptx::cluster_arrive_release();
+        ptx::cluster_wait_acquire();
+        if (ok && !detail::aborted(ab)) {
+          // The tile's 32-column slices are dealt to the parts in order; a slice is finished by the warps of
+          // one half, as without a shared K range.
+          constexpr uint32_t SLICES = TILE_COLS / 32u;
+          for (uint32_t sl = part * SLICES / p.split; sl < (part + 1u) * SLICES / p.split; ++sl) {
+            if ((sl & 1u) != half) continue;
+            const uint32_t col0 = tn * TILE_COLS + sl * 32u;
+            uint32_t x[32], y[32], c[32];
+            if constexpr (!GATED) detail::mx_load_c_words(p, row0 + lane, col0, c);
+            for (uint32_t q = 0; q < p.split; ++q) {
+              const uint32_t peer = ptx::mapa(mine, CTAS == 2 ? q * 2u + rank : q) + sl * (8u * 2048u);
+#pragma unroll
+              for (uint32_t mb = 0; mb < (GATED ? 2u : 1u); ++mb) {
+                float v[8][4];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) ptx::ld_cluster_f32x4(peer + (mb * (BN / 8u) + i) * 2048u, v[i]);
+                uint32_t(&sum)[32] = mb == 0u ? x : y;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  sum[i] = __float_as_uint(q == 0u ? v[i / 4][i % 4] : __uint_as_float(sum[i]) + v[i / 4][i % 4]);
+              }
+            }
+            mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, c, row0, col0, p.n, turn);
+          }
+        }
+      }
+      if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
     }
-    if (p.split > 1u) {
-      __syncwarp();
-      ptx::cluster_arrive_release();  // nobody leaves while a peer may still read its partial sums
+  }
+  if (p.split > 1u) {
+    // The epilogue warps have met their peers once, when the partial sums were in place.
+    __syncwarp();
+    if (warp < 2u || warp == 6u) {
+      ptx::cluster_arrive_release();
       ptx::cluster_wait_acquire();
     }
+    ptx::cluster_arrive_release();  // nobody leaves while a peer may still read its partial sums
+    ptx::cluster_wait_acquire();
   }
 
   // -------------------------------------------------------------- teardown (as in sm100_gemm.cuh)

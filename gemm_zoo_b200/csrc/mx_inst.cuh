@@ -45,9 +45,18 @@ MxEntry mx_entry(bool gated) {
   return {mx_launch<P>, mx_set_attr<P>, P::STAGES, P::SMEM_BYTES};
 }
 
+template <bool NV, int BN, int CTAS>
+MxEntry mx_entry_plain(bool gated) {
+  using P = MxCfg<NV, BN, CTAS, false>;
+  if (gated) return {nullptr, nullptr, 0, 0};
+  return {mx_launch<P>, mx_set_attr<P>, P::STAGES, P::SMEM_BYTES};
+}
+
 template <bool NV>
 MxEntry mx_entry_for(int config, bool gated) {
   switch (config) {
+    case GZ_MX_CFG_PAIR_N128: return mx_entry_plain<NV, 128, 2>(gated);
+    case GZ_MX_CFG_SINGLE_N128: return mx_entry_plain<NV, 128, 1>(gated);
     case GZ_MX_CFG_PAIR: return mx_entry<NV, 256, 2>(gated);
     case GZ_MX_CFG_SINGLE: return mx_entry<NV, 256, 1>(gated);
     case GZ_MX_CFG_SWAP_M16: return mx_entry<NV, 16, 1>(gated);

@@ -16,6 +16,7 @@ from .api import ACT_NONE, ACT_SILU, COL_MAJOR, GZ_OK, Epilogue, GzError, ROW_MA
 
 MX_FP4, MX_NVFP4 = 16, 17
 MX_CFG_AUTO, MX_CFG_PAIR, MX_CFG_SINGLE, MX_CFG_SWAP_M16, MX_CFG_SWAP_M32, MX_CFG_SWAP_M64 = 0, 1, 2, 3, 4, 5
+MX_CFG_PAIR_N128, MX_CFG_SINGLE_N128 = 6, 7
 
 EXPORTED_SYMBOLS = [
     "gz_mx_code_pitch", "gz_mx_scale_bytes", "gz_mx_quantize", "gz_mx_dequantize", "gz_mx_desc_validate",

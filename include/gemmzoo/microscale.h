@@ -69,7 +69,9 @@ typedef enum gz_mx_config {
   GZ_MX_CFG_SINGLE = 2,   /* 128 rows x 256 columns (gated: 128 columns) on one CTA */
   GZ_MX_CFG_SWAP_M16 = 3, /* 128 columns x up to 16 / 32 / 64 rows, m <= 16 / 32 / 64 */
   GZ_MX_CFG_SWAP_M32 = 4,
-  GZ_MX_CFG_SWAP_M64 = 5
+  GZ_MX_CFG_SWAP_M64 = 5,
+  GZ_MX_CFG_PAIR_N128 = 6,  /* 256 rows x 128 columns on a CTA pair (not gated) */
+  GZ_MX_CFG_SINGLE_N128 = 7 /* 128 rows x 128 columns on one CTA (not gated) */
 } gz_mx_config;
 
 /* One product  D[m x n] = A[m x k] * B[n x k]^T  of quantised matrices of one format, or a gated one. */
@@ -80,8 +82,8 @@ typedef struct gz_mx_desc {
   int32_t gated;        /* 0: gz_mx_gemm_run, 1: gz_mx_gated_run */
   int32_t device;
   int32_t config;       /* gz_mx_config */
-  int32_t split;        /* CTAs (PAIR: pairs) that share a tile's K range: 1, 2, 4 or 8
-                           (PAIR and gated SINGLE: at most 4); 0 = chosen */
+  int32_t split;        /* CTAs (pair tiles: pairs) that share a tile's K range: 1, 2, 4 or 8
+                           (at most one per 32 output columns of the tile, and eight CTAs); 0 = chosen */
   uint32_t flags;       /* 0 or GZ_FLAG_TEST_WITHHOLD_ACC_READY */
   int64_t m, n, k;
   int64_t pitch_a, pitch_b; /* bytes between rows of codes (gated: pitch_b for gate and up); 0 = packed */

@@ -46,8 +46,8 @@ def test_sizes():
     (dict(format=3), api.GZ_ERR_INVALID_ARG), (dict(out_type=99), api.GZ_ERR_INVALID_ARG),
     (dict(out_type=gz.DT_S8), api.GZ_ERR_UNSUPPORTED), (dict(out_type=FP4), api.GZ_ERR_UNSUPPORTED),
     (dict(out_type=FP4, gated=True), api.GZ_OK), (dict(out_type=NV, gated=True), api.GZ_OK),
-    (dict(config=6), api.GZ_ERR_INVALID_ARG), (dict(split=3), api.GZ_ERR_INVALID_ARG),
-    (dict(config=gz.MX_CFG_PAIR, split=8), api.GZ_ERR_UNSUPPORTED), (dict(config=gz.MX_CFG_SINGLE, split=8, gated=True), api.GZ_ERR_UNSUPPORTED),
+    (dict(config=8), api.GZ_ERR_INVALID_ARG), (dict(config=gz.MX_CFG_PAIR_N128, gated=True), api.GZ_ERR_UNSUPPORTED), (dict(split=3), api.GZ_ERR_INVALID_ARG),
+    (dict(config=gz.MX_CFG_PAIR, split=8), api.GZ_ERR_UNSUPPORTED), (dict(config=gz.MX_CFG_SINGLE_N128, k=4096, split=8), api.GZ_ERR_UNSUPPORTED), (dict(config=gz.MX_CFG_SINGLE, split=8, gated=True), api.GZ_ERR_UNSUPPORTED),
     (dict(config=gz.MX_CFG_SWAP_M16, m=17), api.GZ_ERR_UNSUPPORTED),
     (dict(config=gz.MX_CFG_SWAP_M16, m=4, n=128, split=8), api.GZ_ERR_UNSUPPORTED),   # one K block
     (dict(flags=1), api.GZ_ERR_INVALID_ARG),
@@ -119,9 +119,10 @@ def test_every_choice_can_be_launched(m, n, k, gated):
     for fmt in FORMATS:
         st, i = gz.mx_validate(gz.MxDesc.make(fmt, gz.DT_BF16, m, n, k, gated))
         assert st == api.GZ_OK and i.smem_bytes <= 232448 and i.stages >= 2
-        ctas = 2 if i.config == gz.MX_CFG_PAIR else 1
+        ctas = 2 if i.config in (gz.MX_CFG_PAIR, gz.MX_CFG_PAIR_N128) else 1
+        swapped = i.config in (gz.MX_CFG_SWAP_M16, gz.MX_CFG_SWAP_M32, gz.MX_CFG_SWAP_M64)
         assert i.grid >= 1 and i.grid % (ctas * i.split) == 0 and ctas * i.split <= 8 and i.split <= -(-k // 256)
-        if i.split > 1 or i.config >= gz.MX_CFG_SWAP_M16:
+        if i.split > 1 or swapped:
             assert i.grid == i.tiles * i.split * ctas
         else:
             assert i.grid <= 148
@@ -271,9 +272,11 @@ def _mx(rows, k, fmt, seed, integers=False):
     return q, orc.decode(codes, scales, fmt)
 
 
-CONFIGS = [gz.MX_CFG_PAIR, gz.MX_CFG_SINGLE, gz.MX_CFG_SWAP_M16, gz.MX_CFG_SWAP_M32, gz.MX_CFG_SWAP_M64]
+CONFIGS = [gz.MX_CFG_PAIR, gz.MX_CFG_SINGLE, gz.MX_CFG_PAIR_N128, gz.MX_CFG_SINGLE_N128, gz.MX_CFG_SWAP_M16, gz.MX_CFG_SWAP_M32, gz.MX_CFG_SWAP_M64]
 ROWS = {gz.MX_CFG_PAIR: [1, 200, 300, 520], gz.MX_CFG_SWAP_M16: [1, 13, 16], gz.MX_CFG_SWAP_M32: [1, 17, 32],
-        gz.MX_CFG_SWAP_M64: [33, 64], gz.MX_CFG_SINGLE: [1, 100, 128, 257]}
+        gz.MX_CFG_SWAP_M64: [33, 64], gz.MX_CFG_SINGLE: [1, 100, 128, 257], gz.MX_CFG_PAIR_N128: [1, 300, 512],
+        gz.MX_CFG_SINGLE_N128: [90, 257]}
+GATED_CONFIGS = [c for c in CONFIGS if c not in (gz.MX_CFG_PAIR_N128, gz.MX_CFG_SINGLE_N128)]
 GUARD = 77.0
 
 
@@ -309,7 +312,7 @@ def test_product_of_integers_is_exact(fmt, config):
 @pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_SWAP_M16, 5, 2), (gz.MX_CFG_SWAP_M16, 16, 4), (gz.MX_CFG_SWAP_M16, 1, 8),
                                             (gz.MX_CFG_SWAP_M32, 21, 8), (gz.MX_CFG_SWAP_M64, 50, 4), (gz.MX_CFG_SINGLE, 128, 4),
                                             (gz.MX_CFG_SINGLE, 200, 2), (gz.MX_CFG_PAIR, 300, 2),
-                                            (gz.MX_CFG_PAIR, 100, 4)])
+                                            (gz.MX_CFG_PAIR, 100, 4), (gz.MX_CFG_PAIR_N128, 300, 4), (gz.MX_CFG_SINGLE_N128, 300, 4)])
 def test_shared_k_ranges(fmt, config, m, split):
     for n, k in [(130, 256 * split), (256, 256 * split + 900), (300, 4096)]:
         a, av = _mx(m, k, fmt, 1, True)
@@ -321,6 +324,8 @@ def test_shared_k_ranges(fmt, config, m, split):
         plan(a, b, None, d, 1.0, 0.0)
         assert plan.device_status()[0] == 0
         assert np.array_equal(d.cpu().double().numpy(), av @ bv.T) and _guards_intact(full, m, n)
+        if config not in GATED_CONFIGS:
+            continue
         plan = gz.MxGated(m, n, k, fmt, torch.float32, activation=gz.ACT_RELU, config=config, split=split, wait_limit_ns=200_000_000)
         plan(a, b, u, d, 2.0 ** -8, 2.0 ** -8)
         assert plan.device_status()[0] == 0
@@ -335,7 +340,7 @@ def _tolerance(want, s, k, dtype):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("config,m", [(gz.MX_CFG_PAIR, 300), (gz.MX_CFG_SWAP_M16, 9), (gz.MX_CFG_SINGLE, 130), (gz.MX_CFG_AUTO, 70)])
+@pytest.mark.parametrize("config,m", [(gz.MX_CFG_PAIR, 300), (gz.MX_CFG_SWAP_M16, 9), (gz.MX_CFG_SINGLE, 130), (gz.MX_CFG_PAIR_N128, 300), (gz.MX_CFG_AUTO, 70)])
 def test_product_epilogue_terms(fmt, dtype, config, m):
     """alpha, beta (C apart from D and in place), bias, row and column scales; rows of D that TMA can and cannot store."""
     for n, k, ldd in [(264, 700, 264), (301, 1025, 303)]:
@@ -391,7 +396,7 @@ def test_activations(act, config, m):
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("config", CONFIGS)
+@pytest.mark.parametrize("config", GATED_CONFIGS)
 def test_gated_product_shapes(fmt, config):
     """relu of integers: the gated product is exact in fp32 (|gate| and |up| below 2^12)."""
     for m in ROWS[config]:
@@ -413,7 +418,7 @@ def test_gated_product_shapes(fmt, config):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("out", FORMATS)
-@pytest.mark.parametrize("config", CONFIGS)
+@pytest.mark.parametrize("config", GATED_CONFIGS)
 def test_gated_product_quantised_output(fmt, out, config):
     """Integer data: the fp32 values are exact, so codes and scales are compared bit for bit; scale rows and blocks
     that do not exist are 0, and nothing beyond a row's codes is written."""
