@@ -8,11 +8,12 @@
 namespace {
 
 template <class K>
-cudaError_t launch(K kernel, const gz::mx::QuantParams& p, dim3 grid, int threads, cudaStream_t stream) {
+cudaError_t launch(K kernel, const gz::mx::QuantParams& p, dim3 grid, int threads, cudaStream_t stream, int smem = 0) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -31,7 +32,7 @@ dim3 grid_of(int64_t rows, int64_t pieces) {
 // Row layout: the 16-element chunks of a row (`chunks`, in whole words of `word`) over equal pieces of
 // at most 256 threads, and as many rows as fit a block of 256.
 template <class K>
-cudaError_t launch_rows(K kernel, gz::mx::QuantParams p, int64_t rows, int64_t chunks, int64_t word, cudaStream_t stream) {
+cudaError_t launch_rows(K kernel, gz::mx::QuantParams p, int64_t rows, int64_t chunks, int64_t word, cudaStream_t stream, int smem = 0) {
   const int64_t pieces = (chunks + 255) / 256;
   const int64_t threads = ((chunks + pieces - 1) / pieces + word - 1) / word * word;
   p.row_threads = static_cast<uint32_t>(threads);
@@ -39,7 +40,7 @@ cudaError_t launch_rows(K kernel, gz::mx::QuantParams p, int64_t rows, int64_t c
   p.block_rows = static_cast<uint32_t>(256 / threads);
   const int64_t per_block = static_cast<int64_t>(p.block_rows) * gz::mx::ROWS_PER_THREAD;
   return launch(kernel, p, grid_of((rows + per_block - 1) / per_block, pieces),
-                static_cast<int>((p.block_rows * threads + 31) / 32 * 32), stream);
+                static_cast<int>((p.block_rows * threads + 31) / 32 * 32), stream, smem);
 }
 
 template <typename T, bool NV>
@@ -52,7 +53,8 @@ cudaError_t quantize(bool cols, const gz::mx::QuantParams& p, cudaStream_t strea
 }
 template <typename T, bool NV>
 cudaError_t dequantize(bool cols, const gz::mx::QuantParams& p, cudaStream_t stream) {
-  if (!cols) return launch_rows(gz::mx::dequantize_rows_kernel<T, NV>, p, p.rows, (p.k + 15) / 16, 1, stream);
+  if (!cols) return launch_rows(gz::mx::dequantize_rows_kernel<T, NV>, p, p.rows, (p.k + 15) / 16, 1, stream,
+                                p.vec ? 0 : 256 * 16 * static_cast<int>(sizeof(T)));
   using Tile = gz::mx::ColTile<T>;
   return launch(gz::mx::dequantize_cols_kernel<T, NV>, p,
                 grid_of((p.rows + Tile::ROWS - 1) / Tile::ROWS, (p.k + gz::mx::COL_K - 1) / gz::mx::COL_K), Tile::THREADS, stream);

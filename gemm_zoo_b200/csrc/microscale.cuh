@@ -58,8 +58,8 @@ gz_status mx_quant_params(gz::mx::QuantParams* p, const void* values, int type, 
   p->groups = mx_groups(format, k);
   p->multiplier = multiplier;
   p->unit = multiplier == 1.0f ? 1u : 0u;
-  const uintptr_t vec = cols ? 16 : 32;  // bytes per access of the two kernels
-  p->vec = (mx_aligned(values, vec) && (ld * size) % (int64_t)vec == 0) ? 1u : 0u;
+  for (const int bytes : {32, 16})  // the widest access that every row allows
+    if (p->vec == 0 && mx_aligned(values, bytes) && (ld * size) % bytes == 0) p->vec = (uint32_t)bytes;
   return GZ_OK;
 }
 
@@ -142,27 +142,38 @@ int64_t mx_resident(const MxShape& s, int cluster, int sm_count) {
   return s.swap() ? 2 * sms : sms;
 }
 
-// Clocks that a configuration is estimated to take; see DESIGN for what the constants were fitted to.
+// Microseconds that a configuration is estimated to take: a fixed part, the K blocks of the longest
+// CTA at the pace of its tile, what handing over a shared K range costs, and never less than the
+// operands take from HBM.  Fitted to graph-timed sweeps of every tile and split over 29 shapes (m 1 to
+// 8192, n 777 to 14336, k 300 to 14336, plain and gated); the pick is the fastest or within 8 % of it.
 double mx_cost(const MxProblem& pr, const MxShape& s, int split, int sm_count) {
-  const int64_t tiles = mx_tiles(pr, s), k_blocks = cdiv(pr.d.k, 256);
-  const bool nv = pr.d.format == GZ_MX_NVFP4;
-  const double mb = (s.swap() && pr.d.gated) ? 2.0 : 1.0;
-  const double bytes = (128.0 * mb + double(s.bn) / s.ctas) * 128.0 + 512.0 * (nv ? 4 : 2) * (mb + (s.bn > 128 ? 2 : 1));
-  const int64_t slots = mx_resident(s, s.ctas * split, sm_count) / (s.ctas * split);  // clusters
+  const int64_t tiles = mx_tiles(pr, s);
+  const bool nv = pr.d.format == GZ_MX_NVFP4, gated = pr.d.gated != 0, quantised = pr.out_size == 0;
+  const int64_t slots = mx_resident(s, s.ctas * split, sm_count) / (s.ctas * split);  // clusters at a time
   if (slots <= 0) return 1e30;
-  const double waves = double(cdiv(tiles, slots));
-  const double blocks = double(cdiv(k_blocks, split));
-  // clocks per K block: the MMAs; the fill from L2 (and, for all CTAs together, from HBM)
-  const double mma = s.swap() ? 200.0 * mb : s.bn == 256 ? 512.0 : s.ctas == 2 ? 300.0 : 330.0;
-  const double active = double(tiles * s.ctas * split < slots * s.ctas * split ? tiles * s.ctas * split : slots * s.ctas * split);
-  const double per_sm = s.swap() && active > sm_count ? 2.0 : 1.0;
-  double per_block = bytes / 60.0 * per_sm;
-  if (mma > per_block) per_block = mma;
-  if (s.swap() && bytes * active / 3400.0 > per_block) per_block = bytes * active / 3400.0;
-  const double finish = s.swap() ? 600.0 + 12.0 * double(pr.d.m) * mb / split : 12.0 * s.bn + (split > 1 ? 30.0 * s.bn : 0.0);
-  const double fixed = 4000.0 + (s.ctas == 2 ? 1500.0 : 0.0) + (split > 1 ? 1500.0 : 0.0);
-  if (s.swap()) return waves * (blocks * per_block + finish) + fixed;
-  return waves * (blocks * per_block + 300.0) + finish + fixed;
+  const double waves = double(cdiv(tiles, slots)), blocks = double(cdiv(cdiv(pr.d.k, 256), split));
+  const double b_bytes = double(pr.d.n) * double(pr.d.k) * (nv ? 0.5625 : 0.53125) * (gated ? 2 : 1);
+  const double hbm = b_bytes / 6.3e6;
+  double fixed, per_block, hand_over, per_wave;
+  if (s.swap()) {
+    fixed = 3.0 + (pr.d.m > 32 ? 0.07 : 0.045) * double(pr.d.m) / split * (gated ? 1.5 : 1.0) * (quantised ? 1.5 : 1.0);
+    per_block = !gated ? 0.28 : nv ? 0.9 : 0.6;  // a gated ring holds two or three stages
+    hand_over = split > 1 ? 0.6 : 0.0;
+    per_wave = 0.3;
+  } else if (s.bn == 256) {
+    fixed = (s.ctas == 2 ? 6.0 : 6.3) + (quantised ? 1.5 : 0.0);
+    per_block = s.ctas == 2 ? 0.308 : 0.47;
+    hand_over = split > 1 ? 3.0 + 0.3 * split : 0.0;
+    per_wave = 0.8;
+  } else {
+    fixed = s.ctas == 2 ? 4.3 : 4.9;
+    per_block = s.ctas == 2 ? 0.267 : tiles * split * 2 <= sm_count ? 0.27 : 0.347;
+    hand_over = split > 1 ? (s.ctas == 2 ? 1.45 * split : 1.1 * split - 1.1) : 0.0;
+    per_wave = 0.6;
+  }
+  double stream = waves * (blocks * per_block + per_wave);
+  if (stream < 1.2 * hbm) stream = 1.2 * hbm;
+  return fixed + hand_over + stream;
 }
 
 int mx_choose_split(const MxProblem& pr, const MxShape& s, int sm_count, double* cost) {

@@ -19,7 +19,11 @@
 //              one MMA computes both halves and no operand is loaded twice.  Two fp32 accumulators of
 //              256 columns would fill tensor memory and leave no room for scales, so they overlap in 64
 //              columns: [0, 256) and [192, 448).  The epilogue reads the shared 64 columns first and
-//              the next tile's main loop starts while it works on the other 192.
+//              the next tile's main loop starts while it works on the other 192.  The tensor pipe idles
+//              for about 1,500 clocks per tile (two signals and the first MMA's way through the pipe);
+//              running ahead with the half that overlaps nothing needs MMAs of 128 columns, which lose
+//              more than that (8192^3: 187 -> 206 us), and a sixth stage in place of half of the
+//              output staging changes nothing.
 //   swapped    few rows of A: B's rows on the 128-lane side (128 features per tile), 16, 32 or 64 rows of
 //              A on the narrow side, so every byte a stage loads is a useful byte of B.  The gated
 //              product keeps two row blocks per stage (gate and up).  One tile per CTA and shared memory

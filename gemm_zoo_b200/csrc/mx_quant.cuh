@@ -26,7 +26,7 @@ struct QuantParams {
   // Row layout: a block takes `block_rows` rows x `row_threads` 16-element chunks (a whole number of
   // scale words); inv_threads = ceil(65536 / row_threads) divides a thread index by row_threads.
   uint32_t row_threads, inv_threads, block_rows;
-  uint32_t vec;   // vector access to the values is legal
+  uint32_t vec;   // bytes that an access to the values may have: 32, 16, or 0 (single values)
   uint32_t unit;  // multiplier == 1
   float multiplier;
 };
@@ -158,9 +158,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
   for (int r = 0; r < ROWS_PER_THREAD; ++r) {
     const int64_t row = row0 + r * p.block_rows;
     const T* src = static_cast<const T*>(p.in) + row * p.ld + k0;
-    if (row < p.rows && k0 + 16 <= p.k && p.vec) {
+    if (row < p.rows && k0 + 16 <= p.k && p.vec == 32u) {
 #pragma unroll
       for (int l = 0; l < WORDS / 8; ++l) load32(src + l * (32 / sizeof(T)), *reinterpret_cast<uint32_t(*)[8]>(&w[r][8 * l]));
+    } else if (row < p.rows && k0 + 16 <= p.k && p.vec == 16u) {
+#pragma unroll
+      for (int l = 0; l < WORDS / 4; ++l)
+        *reinterpret_cast<uint4*>(&w[r][4 * l]) = *reinterpret_cast<const uint4*>(src + l * (16 / sizeof(T)));
     } else {
       T e[16];
 #pragma unroll
@@ -224,9 +228,9 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
     for (int l = 0; l < LINES; ++l) {
       w[l] = make_uint4(0u, 0u, 0u, 0u);
       const int kk = l * STEP + line;
-      if (k0 + kk < p.k) {
+      if (p.vec && k0 + kk < p.k) {
         const T* s = src + static_cast<int64_t>(kk) * p.ld + piece;
-        if (row0 + piece + VEC <= p.rows && p.vec) {
+        if (row0 + piece + VEC <= p.rows) {
           w[l] = *reinterpret_cast<const uint4*>(s);
         } else {
           T* e = reinterpret_cast<T*>(&w[l]);
@@ -237,8 +241,16 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
       }
     }
   }
+  if (p.vec) {
 #pragma unroll
-  for (int l = 0; l < LINES; ++l) *reinterpret_cast<uint4*>(&tile[Tile::at(l * STEP + line, piece)]) = w[l];
+    for (int l = 0; l < LINES; ++l) *reinterpret_cast<uint4*>(&tile[Tile::at(l * STEP + line, piece)]) = w[l];
+  } else {
+    // single values, neighbouring lanes on neighbouring rows
+    for (int i = threadIdx.x; i < Tile::ROWS * COL_K; i += Tile::THREADS) {
+      const int kk = i / Tile::ROWS, r = i % Tile::ROWS;
+      tile[Tile::at(kk, r)] = (k0 + kk < p.k && row0 + r < p.rows) ? src[static_cast<int64_t>(kk) * p.ld + r] : from_float<T>(0.0f);
+    }
+  }
   __syncthreads();
   const uint32_t c = threadIdx.x & 7u;                 // chunk of 16 k
   const int pair = static_cast<int>(threadIdx.x >> 3) * 2;  // first of the two rows
@@ -279,18 +291,20 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
 // once to T.
 template <typename T, bool NV>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(const QuantParams p) {
+  extern __shared__ __align__(16) uint8_t row_buffer[];  // 256 x 16 values where single values are stored, else none
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   int64_t row0, chunk;
-  if (!row_item(p, row0, chunk, ROWS_PER_THREAD) || chunk * 16 >= p.k) return;
+  const bool mine = row_item(p, row0, chunk, ROWS_PER_THREAD) && chunk * 16 < p.k;
+  if (!mine && p.vec) return;
   const int64_t k0 = chunk * 16;
-  uint2 codes[ROWS_PER_THREAD];
-  uint32_t bytes[ROWS_PER_THREAD];
+  uint2 codes[ROWS_PER_THREAD] = {};
+  uint32_t bytes[ROWS_PER_THREAD] = {};
   constexpr int BLOCK = Format<NV>::BLOCK;
 #pragma unroll
   for (int r = 0; r < ROWS_PER_THREAD; ++r) {
     const int64_t row = row0 + r * p.block_rows;
-    if (row < p.rows) {
+    if (mine && row < p.rows) {
       codes[r] = *reinterpret_cast<const uint2*>(p.codes + row * p.pitch + k0 / 2);
       const int64_t block = k0 / BLOCK;
       bytes[r] = __ldg(p.scales + scale_word(row, block >> 2, p.groups) + (block & 3));
@@ -299,28 +313,48 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(const QuantParams 
 #pragma unroll
   for (int r = 0; r < ROWS_PER_THREAD; ++r) {
     const int64_t row = row0 + r * p.block_rows;
-    if (row >= p.rows) break;
     const float s = scale_value<NV>(bytes[r]);
     float v[16];
     unpack8(codes[r].x, *reinterpret_cast<float(*)[8]>(&v[0]));
     unpack8(codes[r].y, *reinterpret_cast<float(*)[8]>(&v[8]));
+    T e[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = v[i] * s * p.multiplier;
-    T* dst = static_cast<T*>(p.out) + row * p.ld + k0;
-    if (k0 + 16 <= p.k && p.vec) {
-      constexpr int STORES = sizeof(T) / 2;
+    for (int i = 0; i < 16; ++i) e[i] = from_float<T>(v[i] * s * p.multiplier);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(e);
+    if (p.vec) {
+      if (row >= p.rows) break;
+      T* dst = static_cast<T*>(p.out) + row * p.ld + k0;
+      constexpr int WORDS = 4 * sizeof(T);
+      if (k0 + 16 <= p.k && p.vec == 32u) {
 #pragma unroll
-      for (int l = 0; l < STORES; ++l) {
-        uint32_t w[8];
-        T* e = reinterpret_cast<T*>(w);
+        for (int l = 0; l < WORDS / 8; ++l) store32(dst + l * (32 / sizeof(T)), *reinterpret_cast<const uint32_t(*)[8]>(&w[8 * l]));
+      } else if (k0 + 16 <= p.k) {
 #pragma unroll
-        for (int i = 0; i < 16 / STORES; ++i) e[i] = from_float<T>(v[l * (16 / STORES) + i]);
-        store32(dst + l * (16 / STORES), w);
+        for (int l = 0; l < WORDS / 4; ++l)
+          *reinterpret_cast<uint4*>(dst + l * (16 / sizeof(T))) = make_uint4(w[4 * l], w[4 * l + 1], w[4 * l + 2], w[4 * l + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k0 + i < p.k) dst[i] = e[i];
       }
     } else {
+      // Rows that start at any value: through shared memory, neighbouring lanes on neighbouring values (16
+      // strided single stores per thread measured 98 us for 16384 x 1000 bf16).
+      T* const buffer = reinterpret_cast<T*>(row_buffer);
+      __syncthreads();  // the previous row has been read out
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (k0 + i < p.k) dst[i] = from_float<T>(v[i]);
+      for (int i = 0; i < 4 * static_cast<int>(sizeof(T)) / 4; ++i)
+        *reinterpret_cast<uint4*>(buffer + threadIdx.x * 16 + i * (16 / sizeof(T))) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      __syncthreads();
+      const int64_t first = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * p.row_threads * 16;  // of the piece
+      const int64_t left = p.k - first;
+      const uint32_t run = static_cast<uint32_t>(left < 0 ? 0 : left < p.row_threads * 16 ? left : p.row_threads * 16);
+      for (uint32_t in = 0; in < p.block_rows; ++in) {
+        const int64_t out_row = static_cast<int64_t>(blockIdx.x) * p.block_rows * ROWS_PER_THREAD + r * p.block_rows + in;
+        if (out_row >= p.rows) break;
+        T* dst = static_cast<T*>(p.out) + out_row * p.ld + first;
+        for (uint32_t i = threadIdx.x; i < run; i += blockDim.x) dst[i] = buffer[in * p.row_threads * 16 + i];
+      }
     }
   }
 }
@@ -368,6 +402,13 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(co
   }
   __syncthreads();
   T* const dst = static_cast<T*>(p.out) + k0 * p.ld + row0;
+  if (!p.vec) {  // single values, neighbouring lanes on neighbouring rows
+    for (int i = threadIdx.x; i < Tile::ROWS * COL_K; i += Tile::THREADS) {
+      const int kk = i / Tile::ROWS, r = i % Tile::ROWS;
+      if (k0 + kk < p.k && row0 + r < p.rows) dst[static_cast<int64_t>(kk) * p.ld + r] = tile[Tile::at(kk, r)];
+    }
+    return;
+  }
   const int line = threadIdx.x / Tile::PER_LINE, piece = (threadIdx.x % Tile::PER_LINE) * VEC;
   constexpr int STEP = Tile::THREADS / Tile::PER_LINE;
 #pragma unroll
@@ -376,7 +417,7 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(co
     if (k0 + kk >= p.k) break;
     const T* e = &tile[Tile::at(kk, piece)];
     T* d = dst + static_cast<int64_t>(kk) * p.ld + piece;
-    if (row0 + piece + VEC <= p.rows && p.vec) {
+    if (row0 + piece + VEC <= p.rows) {
       *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(e);
     } else {
 #pragma unroll

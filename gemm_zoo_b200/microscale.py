@@ -154,23 +154,23 @@ def linear_scales(q: MxMatrix):
     return s.reshape(rg * 128, bg * 4)[:q.rows, :blocks].contiguous()
 
 
-def _matrix_args(x, layout, what):
-    """rows, k, ld of a 2-D tensor in `layout` (row-major: rows x k; column-major: k x rows)."""
+def _refuse_matrix(x, what):
     if x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"{what}: a 2-D CUDA tensor is needed")
-    d0, d1 = x.shape
-    if d1 > 1 and x.stride(1) != 1:
+    if x.shape[1] > 1 and x.stride(1) != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
-    ld = x.stride(0) if d0 > 1 else d1
-    if ld < d1:
-        raise ValueError(f"{what}: rows overlap")
-    return (d0, d1, ld) if layout == ROW_MAJOR else (d1, d0, ld)
+    raise ValueError(f"{what}: rows overlap")
 
 
+# The two calls below cost about as much on the host as on the GPU at the sizes of a single token, so they ask each
+# thing of torch once.
 def mx_quantize(x, format, layout=ROW_MAJOR, multiplier=1.0, out=None, stream=None):
     """Quantise x * multiplier along k (gz_mx_quantize).  x: 2-D, rows x k (ROW_MAJOR) or k x rows (COL_MAJOR).
     Returns `out`, or a new MxMatrix."""
-    rows, k, ld = _matrix_args(x, layout, "mx_quantize")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 2 or not x.is_cuda or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
+        _refuse_matrix(x, "mx_quantize")
+    rows, k = shape if layout == ROW_MAJOR else (shape[1], shape[0])
     if out is None:
         if stream is None or isinstance(stream, int):
             out = MxMatrix.empty(rows, k, format, x.device)
@@ -178,10 +178,11 @@ def mx_quantize(x, format, layout=ROW_MAJOR, multiplier=1.0, out=None, stream=No
             import torch
             with torch.cuda.stream(stream):  # the allocator then knows the memory's stream
                 out = MxMatrix.empty(rows, k, format, x.device)
-    elif out.rows != rows or out.k != k or out.format != format or out.device != x.device.index:
+    elif out.rows != rows or out.k != k or out.format != format or out.device != x.get_device():
         raise ValueError("mx_quantize: out has another size, format or device")
-    st = _bind().gz_mx_quantize(x.data_ptr(), api._torch_dtype_code(x.dtype), layout, ld, rows, k, format, multiplier,
-                                out._codes_ptr, out.pitch, out._scales_ptr, out.device, _stream_handle(stream))
+    st = (_bound or _bind()).gz_mx_quantize(x.data_ptr(), api._torch_dtype_code(x.dtype), layout,
+                                            strides[0] if shape[0] > 1 else 0, rows, k, format, multiplier, out._codes_ptr,
+                                            out.pitch, out._scales_ptr, out.device, _stream_handle(stream))
     if st != GZ_OK:
         raise GzError(st, "gz_mx_quantize")
     return out
@@ -189,11 +190,15 @@ def mx_quantize(x, format, layout=ROW_MAJOR, multiplier=1.0, out=None, stream=No
 
 def mx_dequantize(q: MxMatrix, out, layout=ROW_MAJOR, multiplier=1.0, stream=None):
     """code * scale * multiplier into `out` (gz_mx_dequantize), a 2-D tensor in `layout`.  Returns `out`."""
-    rows, k, ld = _matrix_args(out, layout, "mx_dequantize")
-    if q.rows != rows or q.k != k or q.device != out.device.index:
+    shape, strides = out.shape, out.stride()
+    if len(shape) != 2 or not out.is_cuda or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
+        _refuse_matrix(out, "mx_dequantize")
+    rows, k = shape if layout == ROW_MAJOR else (shape[1], shape[0])
+    if q.rows != rows or q.k != k or q.device != out.get_device():
         raise ValueError("mx_dequantize: out has another size or device")
-    st = _bind().gz_mx_dequantize(q._codes_ptr, q.pitch, q._scales_ptr, q.format, rows, k, multiplier, out.data_ptr(),
-                                  api._torch_dtype_code(out.dtype), layout, ld, q.device, _stream_handle(stream))
+    st = (_bound or _bind()).gz_mx_dequantize(q._codes_ptr, q.pitch, q._scales_ptr, q.format, rows, k, multiplier,
+                                              out.data_ptr(), api._torch_dtype_code(out.dtype), layout,
+                                              strides[0] if shape[0] > 1 else 0, q.device, _stream_handle(stream))
     if st != GZ_OK:
         raise GzError(st, "gz_mx_dequantize")
     return out
@@ -270,7 +275,7 @@ class MxGemm(_MxPlan):
         ep = None
         if bias is not None or row_scale is not None or col_scale is not None or activation != ACT_NONE:
             ep = C.byref(Epilogue.make(bias, row_scale, col_scale, activation))
-        st = _bind().gz_mx_gemm_run(self._h, a._codes_ptr, a._scales_ptr, b._codes_ptr, b._scales_ptr, _ptr(c), _ptr(d),
+        st = _bound.gz_mx_gemm_run(self._h, a._codes_ptr, a._scales_ptr, b._codes_ptr, b._scales_ptr, _ptr(c), _ptr(d),
                                     C.byref(C.c_float(alpha)), C.byref(C.c_float(beta)), ep, _stream_handle(stream))
         if st != GZ_OK:
             raise GzError(st, "gz_mx_gemm_run")
@@ -304,7 +309,7 @@ class MxGated(_MxPlan):
             dp, ds = d._codes_ptr, d._scales_ptr
         else:
             dp, ds = _ptr(d), None
-        st = _bind().gz_mx_gated_run(self._h, a._codes_ptr, a._scales_ptr, gate._codes_ptr, gate._scales_ptr,
+        st = _bound.gz_mx_gated_run(self._h, a._codes_ptr, a._scales_ptr, gate._codes_ptr, gate._scales_ptr,
                                      up._codes_ptr, up._scales_ptr, dp, ds, C.byref(C.c_float(alpha_gate)),
                                      C.byref(C.c_float(alpha_up)), self.activation, out_multiplier,
                                      _stream_handle(stream))
