@@ -248,6 +248,29 @@ def test_quantize_extremes(fmt, layout):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_at_every_border_of_every_scale(fmt):
+    """For each scale a block of its own whose largest value gives that scale, and in it the borders between codes, the
+    fp32 numbers on either side of them, and, in e4m3, largest values at and beside the borders between scales."""
+    scales = orc.E4M3[1:] if fmt == NV else np.ldexp(1.0, np.arange(-100, 100))
+    rows = []
+    for s in scales:
+        for sign in (0, 1, -1):
+            b = (orc.BORDERS * s).astype(np.float32)
+            assert np.array_equal(b.astype(np.float64), orc.BORDERS * s)
+            b = b if sign == 0 else np.nextafter(b, np.float32(np.inf * sign), dtype=np.float32)
+            top = np.float32(6 * s) if fmt == NV else np.float32(7.5 * s)
+            rows.append(np.concatenate([[top], b, -b, np.zeros(1 if fmt == NV else 17, dtype=np.float32)]))
+    if fmt == NV:
+        mid = (orc.E4M3[1:] + orc.E4M3[:-1]) / 2 * 6
+        for top in np.concatenate([np.float32(mid), np.nextafter(np.float32(mid), np.float32(0)), np.nextafter(np.float32(mid), np.float32(1e9))]):
+            rows.append(np.concatenate([[top], np.linspace(0, top, 15)]))
+    x = np.stack(rows).astype(np.float32)
+    q = gz.mx_quantize(torch.from_numpy(x).cuda(), fmt)
+    _check_quantised(x.astype(np.float64), q, fmt)
+
+
+@gpu
 def test_quantize_multiplier():
     x = _values(130, 200, torch.float32, 9) * 0.02
     q = gz.mx_quantize(x.cuda(), NV, multiplier=300.0)
