@@ -22,8 +22,9 @@
 //              the next tile's main loop starts while it works on the other 192.  The tensor pipe idles
 //              for about 1,500 clocks per tile (two signals and the first MMA's way through the pipe);
 //              running ahead with the half that overlaps nothing needs MMAs of 128 columns, which lose
-//              more than that (8192^3: 187 -> 206 us), and a sixth stage in place of half of the
-//              output staging changes nothing.
+//              more than that (8192^3: 187 -> 206 us).  A sixth stage in place of half of the output
+//              staging, the epilogue's parameters held in registers, or one store per 64 columns
+//              change nothing or cost a little.
 //   swapped    few rows of A: B's rows on the 128-lane side (128 features per tile), 16, 32 or 64 rows of
 //              A on the narrow side, so every byte a stage loads is a useful byte of B.  The gated
 //              product keeps two row blocks per stage (gate and up).  One tile per CTA and shared memory
@@ -461,7 +462,7 @@ __device__ __forceinline__ void mx_clear_scale_row(const MxParams& p, uint32_t t
 }
 
 // 32 columns of one row (lane = row) of a row tile, from the sums x (gated: and y) to the output.  c holds
-// the words of C for these columns on entry and those for (next_row, next_col0) on return. 
+// the words of C for these columns on entry and those for next_col0 on return.
 template <class Cfg>
 __device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* tm_d, uint32_t stg, uint32_t lane,
                                                 const uint32_t (&x)[32], const uint32_t (&y)[32], uint32_t (&c)[32],

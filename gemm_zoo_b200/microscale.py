@@ -257,23 +257,50 @@ def _out_code(t):
     return t if isinstance(t, int) else api._torch_dtype_code(t)
 
 
+def _check_dense(name, t, code, rows, cols, ld, device):
+    """A torch tensor given for C or D must be what the plan reads or writes (an address is taken as it is)."""
+    if not hasattr(t, "data_ptr"):
+        return
+    strides = t.stride()
+    if (len(strides) != 2 or t.shape != (rows, cols) or (strides[1] != 1 and cols > 1) or (strides[0] != ld and rows > 1) or
+            api._torch_dtype_code(t.dtype) != code or not t.is_cuda or t.get_device() != device):
+        raise ValueError(f"{name}: expected {rows} x {cols}, rows {ld} elements apart, type {code}, on device {device}; "
+                         f"got {tuple(t.shape)}, strides {strides}, {t.dtype}, {t.device}")
+
+
+def _check_vector(name, t, length, device):
+    if t is None or not hasattr(t, "data_ptr"):
+        return
+    import torch
+    if t.dtype != torch.float32 or t.numel() != length or not t.is_contiguous() or not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{name}: {length} contiguous fp32 values on device {device} are needed")
+
+
 class MxGemm(_MxPlan):
     """D[m x n] = act(alpha * row_scale * col_scale * A B^T + beta * C + bias) for quantised A (m x k) and
-    B (n x k) (gz_mx_gemm_run).  pitch_a / pitch_b: bytes between rows of codes, 0 = packed."""
+    B (n x k) (gz_mx_gemm_run).  pitch_a / pitch_b: bytes between rows of codes, ldc / ldd: elements between rows,
+    0 = packed.  c and d: m x n tensors of the output type with those strides (or addresses)."""
 
     def __init__(self, m, n, k, format, out_dtype, ldc=0, ldd=0, pitch_a=0, pitch_b=0, device=0, config=MX_CFG_AUTO,
                  split=0, flags=0, wait_limit_ns=0):
         super().__init__(MxDesc.make(format, _out_code(out_dtype), m, n, k, False, pitch_a, pitch_b, ldc, ldd, device,
                                      config, split, flags, wait_limit_ns))
-        self._m, self._n, self._k = m, n, k
+        self._m, self._n, self._k, self._ldc, self._ldd = m, n, k, ldc or n, ldd or n
         self._pa, self._pb = pitch_a or code_pitch(k), pitch_b or code_pitch(k)
 
     def __call__(self, a: MxMatrix, b: MxMatrix, c, d, alpha, beta, bias=None, row_scale=None, col_scale=None,
                  activation=ACT_NONE, stream=None):
         self._check("a", a, self._m, self._k, self._pa)
         self._check("b", b, self._n, self._k, self._pb)
+        desc = self.desc
+        _check_dense("d", d, desc.out_type, self._m, self._n, self._ldd, desc.device)
+        if c is not None:
+            _check_dense("c", c, desc.out_type, self._m, self._n, self._ldc, desc.device)
         ep = None
         if bias is not None or row_scale is not None or col_scale is not None or activation != ACT_NONE:
+            _check_vector("bias", bias, self._n, desc.device)
+            _check_vector("row_scale", row_scale, self._m, desc.device)
+            _check_vector("col_scale", col_scale, self._n, desc.device)
             ep = C.byref(Epilogue.make(bias, row_scale, col_scale, activation))
         st = _bound.gz_mx_gemm_run(self._h, a._codes_ptr, a._scales_ptr, b._codes_ptr, b._scales_ptr, _ptr(c), _ptr(d),
                                     C.byref(C.c_float(alpha)), C.byref(C.c_float(beta)), ep, _stream_handle(stream))
@@ -295,7 +322,7 @@ class MxGated(_MxPlan):
         self._pa, self._pb = pitch_a or code_pitch(k), pitch_b or code_pitch(k)
         self._out = self.desc.out_type
         self._quantised = self._out in (MX_FP4, MX_NVFP4)
-        self._pd = ldd or (code_pitch(n) if self._quantised else 0)
+        self._pd = ldd or (code_pitch(n) if self._quantised else n)
 
     def __call__(self, a: MxMatrix, gate: MxMatrix, up: MxMatrix, d, alpha_gate=1.0, alpha_up=1.0, out_multiplier=1.0,
                  stream=None):
@@ -308,6 +335,7 @@ class MxGated(_MxPlan):
                 raise ValueError("d: an MxMatrix of the output's size, format, pitch and device is needed")
             dp, ds = d._codes_ptr, d._scales_ptr
         else:
+            _check_dense("d", d, self._out, self._m, self._n, self._pd, self.desc.device)
             dp, ds = _ptr(d), None
         st = _bound.gz_mx_gated_run(self._h, a._codes_ptr, a._scales_ptr, gate._codes_ptr, gate._scales_ptr,
                                      up._codes_ptr, up._scales_ptr, dp, ds, C.byref(C.c_float(alpha_gate)),

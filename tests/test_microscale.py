@@ -322,7 +322,7 @@ def test_product_of_integers_is_exact(fmt, config):
             b, bv = _mx(n, k, fmt, 2, True)
             full, d = _out(m, n, n + 8, torch.float32)
             plan = gz.MxGemm(m, n, k, fmt, torch.float32, ldd=n + 8, config=config, wait_limit_ns=200_000_000)
-            plan(a, b, None, d, 1.0, 0.0)
+            plan(a, b, None, d[:, :n], 1.0, 0.0)
             assert plan.device_status()[0] == 0
             want = av @ bv.T
             got = d[:, :n].cpu().double().numpy()
@@ -381,7 +381,7 @@ def test_product_epilogue_terms(fmt, dtype, config, m):
             cc = d if inplace else torch.nn.functional.pad(c, (0, 5)).cuda()
             plan = gz.MxGemm(m, n, k, fmt, dtype, ldc=cc.stride(0), ldd=ldd, config=config, wait_limit_ns=200_000_000)
             kw = dict(bias=bias.cuda(), row_scale=rs.cuda(), col_scale=cs.cuda()) if terms else {}
-            plan(a, b, cc if beta else None, d, alpha, beta, **kw)
+            plan(a, b, cc[:, :n] if beta else None, d[:, :n], alpha, beta, **kw)
             assert plan.device_status()[0] == 0
             f = np.outer(rs.double().numpy(), cs.double().numpy()) if terms else 1.0
             want = alpha * f * acc + beta * c.double().numpy() + (bias.double().numpy() if terms else 0.0)
@@ -431,7 +431,7 @@ def test_gated_product_shapes(fmt, config):
             assert np.abs(want).max() < 2 ** 24
             full, d = _out(m, n, n + 4, torch.float32)
             plan = gz.MxGated(m, n, k, fmt, torch.float32, activation=gz.ACT_RELU, ldd=n + 4, config=config, wait_limit_ns=200_000_000)
-            plan(a, g, u, d)
+            plan(a, g, u, d[:, :n])
             assert plan.device_status()[0] == 0
             got = d[:, :n].cpu().double().numpy()
             assert np.array_equal(got, want), (m, n, k, np.argwhere(got != want)[:6])
@@ -479,6 +479,120 @@ def test_nan_stays_in_its_row_and_column(fmt, m):
     want = av @ bv.T
     want[r], want[:, c] = np.nan, np.nan
     assert np.array_equal(d.cpu().double().numpy(), want, equal_nan=True)
+
+
+@gpu
+@pytest.mark.parametrize("config,m", [(gz.MX_CFG_PAIR, 200), (gz.MX_CFG_SWAP_M16, 9)])
+@pytest.mark.parametrize("out", FORMATS)
+def test_nan_in_a_quantised_result_stays_in_its_blocks(config, m, out):
+    n, k = 200, 64
+    a, av = _mx(m, k, FP4, 1, True)
+    g, gv = _mx(n, k, FP4, 2, True)
+    u, uv = _mx(n, k, FP4, 3, True)
+    g.scales[(77 % 32) * 16 + (77 // 32) * 4] = 255  # row 77 of the gate: column 77 of the result
+    q = gz.MxMatrix.empty(m, n, out)
+    gz.MxGated(m, n, k, FP4, out, activation=gz.ACT_NONE, config=config)(a, g, u, q)
+    want = (av @ gv.T) * (av @ uv.T)
+    want[:, 77] = np.nan
+    _check_quantised(want, q, out)
+
+
+@gpu
+@pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_PAIR, 520, 1), (gz.MX_CFG_SWAP_M16, 7, 4), (gz.MX_CFG_SINGLE_N128, 200, 1)])
+def test_one_plan_on_two_streams_and_in_two_graphs(config, m, split):
+    """Calls of one plan may overlap: nothing is kept between them.  Eagerly on two streams, then as two graphs that
+    are replayed at the same time, with operands of their own."""
+    n, k = 1000, 2048
+    ops = [(_mx(m, k, NV, 10 * i + 1, True), _mx(n, k, NV, 10 * i + 2, True)) for i in range(2)]
+    d = [torch.empty(m, n, device="cuda") for _ in range(2)]
+    plan = gz.MxGemm(m, n, k, NV, torch.float32, config=config, split=split)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                plan(ops[i][0][0], ops[i][1][0], None, d[i], 1.0, 0.0, stream=s)
+    torch.cuda.synchronize()
+    want = [ops[i][0][1] @ ops[i][1][1].T for i in range(2)]
+    for i in range(2):
+        assert np.array_equal(d[i].cpu().double().numpy(), want[i])
+        d[i].zero_()
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for _ in range(5):
+                plan(ops[i][0][0], ops[i][1][0], None, d[i], 1.0, 0.0, stream=torch.cuda.current_stream())
+        graphs.append(g)
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert np.array_equal(d[i].cpu().double().numpy(), want[i])
+    assert plan.device_status()[0] == 0
+
+
+@gpu
+def test_padded_pitches_of_the_operands():
+    """Rows of codes further apart than packed, for every operand of every kind of tile; what lies between is never read."""
+    for config, m in [(gz.MX_CFG_PAIR, 260), (gz.MX_CFG_SINGLE, 130), (gz.MX_CFG_SWAP_M32, 20)]:
+        n, k = 150, 330
+        mats = []
+        for i, rows in enumerate((m, n, n)):
+            q, v = _mx(rows, k, NV, i + 1, True)
+            wide = torch.full((rows, ms.code_pitch(k) + 48), 0x77, dtype=torch.uint8, device="cuda")
+            wide[:, :(k + 1) // 2] = q.codes[:, :(k + 1) // 2]
+            mats.append((gz.MxMatrix(wide, q.scales, rows, k, NV), v))
+        p = ms.code_pitch(k) + 48
+        d = torch.empty(m, n, device="cuda")
+        gz.MxGemm(m, n, k, NV, torch.float32, pitch_a=p, pitch_b=p, config=config)(mats[0][0], mats[1][0], None, d, 1.0, 0.0)
+        assert np.array_equal(d.cpu().double().numpy(), mats[0][1] @ mats[1][1].T)
+        gz.MxGated(m, n, k, NV, torch.float32, activation=gz.ACT_NONE, pitch_a=p, pitch_b=p, config=config)(
+            mats[0][0], mats[1][0], mats[2][0], d, 2.0 ** -8, 1.0)
+        want = ((mats[0][1] @ mats[1][1].T) * 2.0 ** -8).astype(np.float32) * (mats[0][1] @ mats[2][1].T).astype(np.float32)
+        assert np.array_equal(d.cpu().numpy(), want)
+
+
+DEBUG_CHILD = """
+import sys
+sys.path.insert(0, {root!r})
+import gemm_zoo_b200.api as api
+api.lib_path = api.debug_lib_path  # before the first lib() call: this process runs the debug build
+import numpy as np
+import torch
+import gemm_zoo_b200 as gz
+from tests import test_microscale as t
+for config, m in [(gz.MX_CFG_PAIR, 300), (gz.MX_CFG_SINGLE, 130), (gz.MX_CFG_PAIR_N128, 300), (gz.MX_CFG_SWAP_M16, 13), (gz.MX_CFG_SWAP_M64, 40)]:
+    for n in (203, 333):
+        a, av = t._mx(m, 300, gz.MX_FP4, 1, True)
+        b, bv = t._mx(n, 300, gz.MX_FP4, 2, True)
+        for dtype in (torch.float32, torch.bfloat16):
+            d = torch.empty(m, n, dtype=dtype, device="cuda")
+            p = gz.MxGemm(m, n, 300, gz.MX_FP4, dtype, config=config)
+            p(a, b, None, d, 1.0, 0.0)
+            assert p.device_status()[0] == 0, p.device_status()
+            assert torch.equal(d.cpu(), torch.from_numpy(av @ bv.T).to(dtype))
+        if config != gz.MX_CFG_PAIR_N128:
+            q = gz.MxMatrix.empty(m, n, gz.MX_NVFP4)
+            p = gz.MxGated(m, n, 300, gz.MX_FP4, gz.MX_NVFP4, activation=gz.ACT_RELU, config=config)
+            p(a, b, b, q, 2.0 ** -8, 2.0 ** -8)
+            assert p.device_status()[0] == 0, p.device_status()
+print("DEBUG OK")
+"""
+
+
+@gpu
+def test_debug_build_refuses_no_store():
+    """The checked build (every plain store of the epilogue checks its coordinates first) refuses nothing."""
+    import subprocess
+    import sys
+    from gemm_zoo_b200 import build as b
+    b.build_lib(debug=True)
+    root = str(api.PKG.parent)
+    r = subprocess.run([sys.executable, "-c", DEBUG_CHILD.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "DEBUG OK" in r.stdout, (r.stdout[-500:], r.stderr[-2000:])
 
 
 @gpu
@@ -556,6 +670,15 @@ def test_python_refusals():
     d = torch.empty(8, 8, device="cuda")
     with pytest.raises(ValueError):
         plan(q, gz.mx_quantize(x[:4], FP4), None, d, 1.0, 0.0)
+    for bad in (d.half(), d[:4], d.cpu(), torch.empty(8, 16, device="cuda")[:, :8], d.t()[:, :4]):
+        with pytest.raises(ValueError):
+            plan(q, q, None, bad, 1.0, 0.0)
+        with pytest.raises(ValueError):
+            plan(q, q, bad, d, 1.0, 1.0)
+    for name in ("bias", "row_scale", "col_scale"):
+        for bad in (torch.zeros(7, device="cuda"), torch.zeros(8, device="cuda").half(), torch.zeros(8), torch.zeros(16, device="cuda")[::2]):
+            with pytest.raises(ValueError):
+                plan(q, q, None, d, 1.0, 0.0, **{name: bad})
     with pytest.raises(gz.GzError) as e:
         plan(q, q, None, d, 1.0, 1.0)  # beta without C
     assert e.value.status == api.GZ_ERR_INVALID_ARG
