@@ -12,7 +12,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import api
-from .api import ACT_NONE, ACT_SILU, COL_MAJOR, GZ_OK, Epilogue, GzError, ROW_MAJOR, _ptr, _stream_handle, lib
+from .api import ACT_NONE, ACT_SILU, GZ_OK, Epilogue, GzError, ROW_MAJOR, _stream_handle, lib
 
 MX_FP4, MX_NVFP4 = 16, 17
 MX_CFG_AUTO, MX_CFG_PAIR, MX_CFG_SINGLE, MX_CFG_SWAP_M16, MX_CFG_SWAP_M32, MX_CFG_SWAP_M64 = 0, 1, 2, 3, 4, 5
@@ -101,7 +101,7 @@ class MxMatrix:
     """A quantised rows x k matrix: `codes` (uint8, rows x pitch bytes) and `scales` (uint8, flat, in tiles of
     128 rows x 4 blocks); the layout is that of include/gemmzoo/microscale.h."""
 
-    __slots__ = ("codes", "scales", "rows", "k", "format", "device", "pitch", "_codes_ptr", "_scales_ptr")
+    __slots__ = ("codes", "scales", "rows", "k", "format", "device", "pitch", "_codes_ptr", "_scales_ptr", "_key")
 
     def __init__(self, codes, scales, rows, k, format):
         import torch
@@ -124,6 +124,7 @@ class MxMatrix:
         self.codes, self.scales, self.rows, self.k, self.format = codes, scales, rows, k, format
         self.device, self.pitch = codes.device.index, pitch
         self._codes_ptr, self._scales_ptr = codes.data_ptr(), scales.data_ptr()
+        self._key = (rows, k, format, pitch, self.device)  # what a plan compares
 
     @classmethod
     def empty(cls, rows, k, format, device="cuda"):
@@ -247,25 +248,45 @@ class _MxPlan:
         except Exception:
             pass
 
-    def _check(self, name, q, rows, k, pitch):
-        if q.rows != rows or q.k != k or q.format != self.desc.format or q.device != self.desc.device or q.pitch != pitch:
-            raise ValueError(f"{name}: expected {rows} x {k}, format {self.desc.format}, pitch {pitch} on device {self.desc.device}, "
-                             f"got {q.rows} x {q.k}, format {q.format}, pitch {q.pitch} on device {q.device}")
+    def _refuse(self, name, q, key):
+        got = getattr(q, "_key", None)
+        raise ValueError(f"{name}: an MxMatrix of (rows, k, format, pitch, device) = {key} is needed, got {got or type(q)}")
 
 
 def _out_code(t):
     return t if isinstance(t, int) else api._torch_dtype_code(t)
 
 
-def _check_dense(name, t, code, rows, cols, ld, device):
-    """A torch tensor given for C or D must be what the plan reads or writes (an address is taken as it is)."""
-    if not hasattr(t, "data_ptr"):
-        return
-    strides = t.stride()
-    if (len(strides) != 2 or t.shape != (rows, cols) or (strides[1] != 1 and cols > 1) or (strides[0] != ld and rows > 1) or
-            api._torch_dtype_code(t.dtype) != code or not t.is_cuda or t.get_device() != device):
-        raise ValueError(f"{name}: expected {rows} x {cols}, rows {ld} elements apart, type {code}, on device {device}; "
-                         f"got {tuple(t.shape)}, strides {strides}, {t.dtype}, {t.device}")
+class _Dense:
+    """What a torch tensor given for C or D must be: the plan reads or writes it by address.  (An address, an int, is taken as
+    it is.)  These checks run in every call, beside kernels of a few microseconds, so they compare prepared values."""
+
+    def __init__(self, name, code, rows, cols, ld, device):
+        import torch
+        self.name, self.ld, self.device = name, ld, device
+        self.shape, self.strides = torch.Size((rows, cols)), (ld, 1)
+        self.dtype = next((t for t, c in _torch_types().items() if c == code), None)
+
+    def address(self, t):
+        if isinstance(t, int):
+            return t
+        if t.stride() != self.strides or t.shape != self.shape or t.dtype is not self.dtype or t.get_device() != self.device:
+            self._look_closer(t)
+        return t.data_ptr()
+
+    def _look_closer(self, t):
+        rows, cols = self.shape
+        ok = (t.shape == self.shape and t.dtype is self.dtype and t.get_device() == self.device and
+              (t.stride(1) == 1 or cols == 1) and (t.stride(0) == self.ld or rows == 1))  # strides of one row mean nothing
+        if not ok:
+            raise ValueError(f"{self.name}: expected {tuple(self.shape)}, rows {self.ld} elements apart, {self.dtype}, on device "
+                             f"{self.device}; got {tuple(t.shape)}, strides {t.stride()}, {t.dtype}, {t.device}")
+
+
+def _torch_types():
+    import torch
+    api._torch_dtype_code(torch.float32)
+    return api._TORCH_DT
 
 
 def _check_vector(name, t, length, device):
@@ -285,25 +306,29 @@ class MxGemm(_MxPlan):
                  split=0, flags=0, wait_limit_ns=0):
         super().__init__(MxDesc.make(format, _out_code(out_dtype), m, n, k, False, pitch_a, pitch_b, ldc, ldd, device,
                                      config, split, flags, wait_limit_ns))
-        self._m, self._n, self._k, self._ldc, self._ldd = m, n, k, ldc or n, ldd or n
-        self._pa, self._pb = pitch_a or code_pitch(k), pitch_b or code_pitch(k)
+        out = self.desc.out_type
+        self._m, self._n, self._device = m, n, device
+        self._a = (m, k, format, pitch_a or code_pitch(k), device)
+        self._b = (n, k, format, pitch_b or code_pitch(k), device)
+        self._c, self._d = _Dense("c", out, m, n, ldc or n, device), _Dense("d", out, m, n, ldd or n, device)
+        self._run = _bound.gz_mx_gemm_run
 
     def __call__(self, a: MxMatrix, b: MxMatrix, c, d, alpha, beta, bias=None, row_scale=None, col_scale=None,
                  activation=ACT_NONE, stream=None):
-        self._check("a", a, self._m, self._k, self._pa)
-        self._check("b", b, self._n, self._k, self._pb)
-        desc = self.desc
-        _check_dense("d", d, desc.out_type, self._m, self._n, self._ldd, desc.device)
-        if c is not None:
-            _check_dense("c", c, desc.out_type, self._m, self._n, self._ldc, desc.device)
+        if getattr(a, "_key", None) != self._a:
+            self._refuse("a", a, self._a)
+        if getattr(b, "_key", None) != self._b:
+            self._refuse("b", b, self._b)
+        dp = self._d.address(d)
+        cp = None if c is None else self._c.address(c)
         ep = None
-        if bias is not None or row_scale is not None or col_scale is not None or activation != ACT_NONE:
-            _check_vector("bias", bias, self._n, desc.device)
-            _check_vector("row_scale", row_scale, self._m, desc.device)
-            _check_vector("col_scale", col_scale, self._n, desc.device)
+        if activation != ACT_NONE or bias is not None or row_scale is not None or col_scale is not None:
+            _check_vector("bias", bias, self._n, self._device)
+            _check_vector("row_scale", row_scale, self._m, self._device)
+            _check_vector("col_scale", col_scale, self._n, self._device)
             ep = C.byref(Epilogue.make(bias, row_scale, col_scale, activation))
-        st = _bound.gz_mx_gemm_run(self._h, a._codes_ptr, a._scales_ptr, b._codes_ptr, b._scales_ptr, _ptr(c), _ptr(d),
-                                    C.byref(C.c_float(alpha)), C.byref(C.c_float(beta)), ep, _stream_handle(stream))
+        st = self._run(self._h, a._codes_ptr, a._scales_ptr, b._codes_ptr, b._scales_ptr, cp, dp, C.byref(C.c_float(alpha)),
+                       C.byref(C.c_float(beta)), ep, _stream_handle(stream))
         if st != GZ_OK:
             raise GzError(st, "gz_mx_gemm_run")
 
@@ -318,28 +343,29 @@ class MxGated(_MxPlan):
         super().__init__(MxDesc.make(format, _out_code(out_dtype), m, n, k, True, pitch_a, pitch_b, 0, ldd, device,
                                      config, split, flags, wait_limit_ns))
         self.activation = activation
-        self._m, self._n, self._k = m, n, k
-        self._pa, self._pb = pitch_a or code_pitch(k), pitch_b or code_pitch(k)
-        self._out = self.desc.out_type
-        self._quantised = self._out in (MX_FP4, MX_NVFP4)
-        self._pd = ldd or (code_pitch(n) if self._quantised else n)
+        out = self.desc.out_type
+        self._a = (m, k, format, pitch_a or code_pitch(k), device)
+        self._b = (n, k, format, pitch_b or code_pitch(k), device)
+        self._quantised = out in (MX_FP4, MX_NVFP4)
+        self._d = (m, n, out, ldd or code_pitch(n), device) if self._quantised else _Dense("d", out, m, n, ldd or n, device)
+        self._run = _bound.gz_mx_gated_run
 
     def __call__(self, a: MxMatrix, gate: MxMatrix, up: MxMatrix, d, alpha_gate=1.0, alpha_up=1.0, out_multiplier=1.0,
                  stream=None):
-        self._check("a", a, self._m, self._k, self._pa)
-        self._check("gate", gate, self._n, self._k, self._pb)
-        self._check("up", up, self._n, self._k, self._pb)
+        if getattr(a, "_key", None) != self._a:
+            self._refuse("a", a, self._a)
+        if getattr(gate, "_key", None) != self._b:
+            self._refuse("gate", gate, self._b)
+        if getattr(up, "_key", None) != self._b:
+            self._refuse("up", up, self._b)
         if self._quantised:
-            if not isinstance(d, MxMatrix) or (d.rows, d.k, d.format, d.device, d.pitch) != (
-                    self._m, self._n, self._out, self.desc.device, self._pd):
-                raise ValueError("d: an MxMatrix of the output's size, format, pitch and device is needed")
+            if getattr(d, "_key", None) != self._d:
+                self._refuse("d", d, self._d)
             dp, ds = d._codes_ptr, d._scales_ptr
         else:
-            _check_dense("d", d, self._out, self._m, self._n, self._pd, self.desc.device)
-            dp, ds = _ptr(d), None
-        st = _bound.gz_mx_gated_run(self._h, a._codes_ptr, a._scales_ptr, gate._codes_ptr, gate._scales_ptr,
-                                     up._codes_ptr, up._scales_ptr, dp, ds, C.byref(C.c_float(alpha_gate)),
-                                     C.byref(C.c_float(alpha_up)), self.activation, out_multiplier,
-                                     _stream_handle(stream))
+            dp, ds = self._d.address(d), None
+        st = self._run(self._h, a._codes_ptr, a._scales_ptr, gate._codes_ptr, gate._scales_ptr, up._codes_ptr, up._scales_ptr,
+                       dp, ds, C.byref(C.c_float(alpha_gate)), C.byref(C.c_float(alpha_up)), self.activation, out_multiplier,
+                       _stream_handle(stream))
         if st != GZ_OK:
             raise GzError(st, "gz_mx_gated_run")

@@ -652,6 +652,9 @@ def test_feed_forward_chain(fmt, m):
 def test_python_refusals():
     x = torch.zeros(8, 64, device="cuda")
     q = gz.mx_quantize(x, FP4)
+    for bad in (torch.zeros(64, device="cuda"), torch.zeros(8, 8, 8, device="cuda"), torch.zeros(8, 1, device="cuda").expand(8, 64)):
+        with pytest.raises(ValueError):
+            gz.mx_quantize(bad, FP4)
     with pytest.raises(ValueError):
         gz.mx_quantize(x.cpu(), FP4)
     with pytest.raises(ValueError):
@@ -686,8 +689,11 @@ def test_python_refusals():
         plan(q, q, None, d.data_ptr() + 1, 1.0, 0.0)
     assert e.value.status == api.GZ_ERR_MISALIGNED
     h = gz.MxGated(8, 8, 64, FP4, NV)
+    for bad in (d, q, None, 3):
+        with pytest.raises(ValueError):
+            h(q, q, q, bad)
     with pytest.raises(ValueError):
-        h(q, q, q, d)
+        plan(x, q, None, d, 1.0, 0.0)
     one = C.c_float(1.0)
     L = ms._bind()
     args = (q._codes_ptr, q._scales_ptr) * 3
