@@ -48,15 +48,16 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 32 bytes at a 32-byte aligned address.
+// 32 bytes at a 32-byte aligned address.  What is quantised is read once and what is decoded written once, so
+// both may leave the L2 first: quantise and decode in turn 16384 x 4096 bf16 57.7 -> 52.3 us.
 __device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8]) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+  asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                : "l"(p)
                : "memory");
 }
 __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+  asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
   if (p.vec && k0 + COL_K <= p.k && row0 + Tile::ROWS <= p.rows) {
 #pragma unroll
     for (int l = 0; l < LINES; ++l)
-      w[l] = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(l * STEP + line) * p.ld + piece);
+      w[l] = __ldcs(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(l * STEP + line) * p.ld + piece));
   } else {
 #pragma unroll
     for (int l = 0; l < LINES; ++l) {
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(co
     const T* e = &tile[Tile::at(kk, piece)];
     T* d = dst + static_cast<int64_t>(kk) * p.ld + piece;
     if (row0 + piece + VEC <= p.rows) {
-      *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(e);
+      __stcs(reinterpret_cast<uint4*>(d), *reinterpret_cast<const uint4*>(e));
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
