@@ -142,10 +142,11 @@ int64_t mx_resident(const MxShape& s, int cluster, int sm_count) {
   return s.swap() ? 2 * sms : sms;
 }
 
-// Microseconds that a configuration is estimated to take: a fixed part, the K blocks of the longest
-// CTA at the pace of its tile, what handing over a shared K range costs, and never less than the
-// operands take from HBM.  Fitted to graph-timed sweeps of every tile and split over 29 shapes (m 1 to
-// 8192, n 777 to 14336, k 300 to 14336, plain and gated); the pick is the fastest or within 8 % of it.
+// Microseconds that a configuration is estimated to take: a fixed part, the K blocks of the longest CTA at
+// the pace of its tile, what handing over a shared K range costs, and never less than B takes from HBM
+// (of which a swapped CTA, with its ring of 110 KB, draws 43 GB/s under load).  Fitted to graph-timed
+// sweeps of every tile and split over 129 shapes, plain and gated, m 1 to 8192; over 100 other random shapes the
+// pick lost 1.5 % on the best configuration on average and 15 % at worst.
 double mx_cost(const MxProblem& pr, const MxShape& s, int split, int sm_count) {
   const int64_t tiles = mx_tiles(pr, s);
   const bool nv = pr.d.format == GZ_MX_NVFP4, gated = pr.d.gated != 0, quantised = pr.out_size == 0;
@@ -153,27 +154,29 @@ double mx_cost(const MxProblem& pr, const MxShape& s, int split, int sm_count) {
   if (slots <= 0) return 1e30;
   const double waves = double(cdiv(tiles, slots)), blocks = double(cdiv(cdiv(pr.d.k, 256), split));
   const double b_bytes = double(pr.d.n) * double(pr.d.k) * (nv ? 0.5625 : 0.53125) * (gated ? 2 : 1);
-  const double hbm = b_bytes / 6.3e6;
-  double fixed, per_block, hand_over, per_wave;
+  const double m = double(pr.d.m);
+  double fixed, per_block, hand_over = 0.0, per_wave, hbm = b_bytes / 6.3e6;
   if (s.swap()) {
-    fixed = 3.0 + (pr.d.m > 32 ? 0.07 : 0.045) * double(pr.d.m) / split * (gated ? 1.5 : 1.0) * (quantised ? 1.5 : 1.0);
+    // parking is every CTA's, finishing is shared
+    fixed = 3.3 + 0.04 * m * (gated ? 1.5 : 1.0) + 0.04 * m / split * (gated ? 1.5 : 1.0) * (quantised ? 1.5 : 1.0);
     per_block = !gated ? 0.28 : nv ? 0.9 : 0.6;  // a gated ring holds two or three stages
-    hand_over = split > 1 ? 0.6 : 0.0;
+    if (split > 1) hand_over = 0.6;
     per_wave = 0.3;
+    const double ctas = double(tiles) * split, drawn = 43e3 * (ctas < 2.0 * sm_count ? ctas : 2.0 * sm_count);
+    if (drawn < 6.3e6) hbm = b_bytes / drawn;
   } else if (s.bn == 256) {
-    fixed = (s.ctas == 2 ? 6.0 : 6.3) + (quantised ? 1.5 : 0.0);
-    per_block = s.ctas == 2 ? 0.308 : 0.47;
-    hand_over = split > 1 ? 3.0 + 0.3 * split : 0.0;
+    fixed = (s.ctas == 2 ? 5.4 : 4.9) + (quantised ? 3.0 : gated ? 1.0 : 0.0);
+    per_block = s.ctas == 2 ? 0.318 : 0.5;
+    if (split > 1) hand_over = split == 2 ? 3.2 : 6.0;
     per_wave = 0.8;
   } else {
-    fixed = s.ctas == 2 ? 4.3 : 4.9;
-    per_block = s.ctas == 2 ? 0.267 : tiles * split * 2 <= sm_count ? 0.27 : 0.347;
-    hand_over = split > 1 ? (s.ctas == 2 ? 1.45 * split : 1.1 * split - 1.1) : 0.0;
+    fixed = s.ctas == 2 ? 3.9 : 3.5;
+    per_block = s.ctas == 2 ? 0.267 : tiles * split * 2 <= sm_count ? 0.29 : 0.38;
+    if (split > 1) hand_over = 0.95 * split;
     per_wave = 0.6;
   }
-  double stream = waves * (blocks * per_block + per_wave);
-  if (stream < 1.2 * hbm) stream = 1.2 * hbm;
-  return fixed + hand_over + stream;
+  const double stream = waves * (blocks * per_block + per_wave);
+  return fixed + hand_over + (stream > hbm ? stream : hbm);
 }
 
 int mx_choose_split(const MxProblem& pr, const MxShape& s, int sm_count, double* cost) {
