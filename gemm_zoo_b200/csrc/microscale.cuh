@@ -48,6 +48,7 @@ gz_status mx_quant_params(gz::mx::QuantParams* p, const void* values, int type, 
   if (ld < (cols ? rows : k) || pitch < gz_mx_code_pitch(k) || pitch % 16 != 0) return GZ_ERR_INVALID_ARG;
   const int size = dtype_size(type);
   if (!mx_span_ok(cols ? k : rows, ld) || !mx_span_ok(rows, pitch)) return GZ_ERR_TOO_LARGE;
+  if (values == codes || values == scales || codes == scales) return GZ_ERR_INVALID_ARG;  // nothing is converted in place
   if (!mx_aligned(values, size) || !mx_aligned(codes, 16) || !mx_aligned(scales, 16)) return GZ_ERR_MISALIGNED;
   std::memset(p, 0, sizeof(*p));
   p->rows = rows;
@@ -465,6 +466,8 @@ GZ_API gz_status gz_mx_gemm_run(gz_mx_plan* pl, const void* a, const void* a_sca
   if (*beta != 0.0f && !c) return GZ_ERR_INVALID_ARG;
   const gz_mx_desc& ds = pl->pr.d;
   const int size = pl->pr.out_size;
+  if (d == a || d == b || d == a_scales || d == b_scales) return GZ_ERR_INVALID_ARG;
+  if (*beta != 0.0f && c == d && ds.ldc != ds.ldd && ds.m > 1) return GZ_ERR_INVALID_ARG;  // other CTAs' rows of C
   if (!mx_aligned(a, 16) || !mx_aligned(a_scales, 16) || !mx_aligned(b, 16) || !mx_aligned(b_scales, 16) ||
       !mx_aligned(d, size) || !mx_aligned(c, size))
     return GZ_ERR_MISALIGNED;
@@ -498,6 +501,9 @@ GZ_API gz_status gz_mx_gated_run(gz_mx_plan* pl, const void* a, const void* a_sc
     return GZ_ERR_INVALID_ARG;
   const bool quantised = pl->pr.out_size == 0;
   if (quantised != (d_scales != nullptr)) return GZ_ERR_INVALID_ARG;
+  for (const void* in : {a, a_scales, gate, gate_scales, up, up_scales})  // read while others write
+    if (d == in || (d_scales && d_scales == in)) return GZ_ERR_INVALID_ARG;
+  if (d == d_scales) return GZ_ERR_INVALID_ARG;
   if (quantised && (!(std::fabs(out_multiplier) <= 3.4028234e38f) || out_multiplier == 0.0f)) return GZ_ERR_INVALID_ARG;
   if (!mx_aligned(a, 16) || !mx_aligned(a_scales, 16) || !mx_aligned(gate, 16) || !mx_aligned(gate_scales, 16) ||
       !mx_aligned(up, 16) || !mx_aligned(up_scales, 16) || !mx_aligned(d, quantised ? 16 : pl->pr.out_size) ||

@@ -798,7 +798,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
           continue;
         }
         live = true;
-        const bool ok = detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0);
+        const bool ok = __all_sync(0xFFFFFFFFu, detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0));
         if (ok) {
           ptx::tc_fence_after_sync();
 #pragma unroll 1
@@ -846,7 +846,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
           auto group_col = [&](uint32_t s) { return tile_col + ((it & 1u) ? s : (s + GROUPS - 1u) % GROUPS) * 64u; };
           uint32_t c[32];
           if constexpr (!GATED) detail::mx_load_c_words(p, row0 + lane, group_col(0), c);
-          if (!detail::wait(acc_full_bar, it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0)) break;
+          if (!__all_sync(0xFFFFFFFFu, detail::wait(acc_full_bar, it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0))) break;
           ptx::tc_fence_after_sync();
           const uint32_t acc = lanes + (it & 1u) * Cfg::ACC_STRIDE;
 #pragma unroll 1
@@ -874,7 +874,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
         tile_coords(p.grid, cluster, tm, tn);
         const uint32_t row0 = (tm * CTAS + rank) * 128u + quad * 32u;
         const uint32_t mine = base + (quad * 32u + lane) * 16u;
-        const bool ok = detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0);
+        const bool ok = __all_sync(0xFFFFFFFFu, detail::wait(acc_full_bar, 0, ab, WAIT_EPILOGUE_TMEM_FULL, cluster, 0));
         if (ok) {
           ptx::tc_fence_after_sync();
 #pragma unroll 1

@@ -99,9 +99,15 @@ def scale_bytes(format: int, rows: int, k: int) -> int:
 
 class MxMatrix:
     """A quantised rows x k matrix: `codes` (uint8, rows x pitch bytes) and `scales` (uint8, flat, in tiles of
-    128 rows x 4 blocks); the layout is that of include/gemmzoo/microscale.h."""
+    128 rows x 4 blocks); the layout is that of include/gemmzoo/microscale.h.  The attributes are not replaced
+    after construction, which checked them together; the tensors' contents are the caller's."""
 
-    __slots__ = ("codes", "scales", "rows", "k", "format", "device", "pitch", "_codes_ptr", "_scales_ptr", "_key")
+    __slots__ = ("_codes", "_scales", "_key")  # _key: (rows, k, format, pitch, device), what a plan compares
+    codes, scales = property(lambda self: self._codes), property(lambda self: self._scales)
+    rows, k = property(lambda self: self._key[0]), property(lambda self: self._key[1])
+    format, pitch = property(lambda self: self._key[2]), property(lambda self: self._key[3])
+    device = property(lambda self: self._key[4])
+    _codes_ptr, _scales_ptr = property(lambda self: self._codes.data_ptr()), property(lambda self: self._scales.data_ptr())
 
     def __init__(self, codes, scales, rows, k, format):
         import torch
@@ -114,17 +120,17 @@ class MxMatrix:
         if not (codes.is_cuda and codes.device == scales.device):
             raise ValueError("MxMatrix: codes and scales must live on one CUDA device")
         pitch = codes.stride(0) if codes.dim() == 2 and rows > 1 else codes.shape[-1]
-        if codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] < code_pitch(k) or codes.stride(1) != 1 or pitch % 16:
-            raise ValueError(f"MxMatrix: codes must be rows x at least {code_pitch(k)} bytes, contiguous along a row, "
-                             "rows a multiple of 16 bytes apart")
+        packed = code_pitch(k)
+        if (codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] < packed or codes.stride(1) != 1 or pitch % 16 or
+                pitch < packed):
+            raise ValueError(f"MxMatrix: codes must be rows x at least {packed} bytes, contiguous along a row, "
+                             "rows a multiple of 16 bytes apart that do not overlap")
         if not scales.is_contiguous() or scales.numel() < need:
             raise ValueError(f"MxMatrix: scales must be {need} contiguous bytes")
         if codes.data_ptr() % 16 or scales.data_ptr() % 16:
             raise ValueError("MxMatrix: codes and scales must be 16-byte aligned")
-        self.codes, self.scales, self.rows, self.k, self.format = codes, scales, rows, k, format
-        self.device, self.pitch = codes.device.index, pitch
-        self._codes_ptr, self._scales_ptr = codes.data_ptr(), scales.data_ptr()
-        self._key = (rows, k, format, pitch, self.device)  # what a plan compares
+        self._codes, self._scales = codes, scales
+        self._key = (rows, k, format, pitch, codes.get_device())
 
     @classmethod
     def empty(cls, rows, k, format, device="cuda"):
@@ -167,23 +173,25 @@ def _refuse_matrix(x, what):
 # thing of torch once.
 def mx_quantize(x, format, layout=ROW_MAJOR, multiplier=1.0, out=None, stream=None):
     """Quantise x * multiplier along k (gz_mx_quantize).  x: 2-D, rows x k (ROW_MAJOR) or k x rows (COL_MAJOR).
-    Returns `out`, or a new MxMatrix."""
+    Returns `out`, or a new MxMatrix.  stream: None is the default stream, as everywhere in this package."""
     shape, strides = x.shape, x.stride()
     if len(shape) != 2 or not x.is_cuda or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
         _refuse_matrix(x, "mx_quantize")
     rows, k = shape if layout == ROW_MAJOR else (shape[1], shape[0])
     if out is None:
-        if stream is None or isinstance(stream, int):
-            out = MxMatrix.empty(rows, k, format, x.device)
+        import torch
+        if stream is None:
+            on = torch.cuda.default_stream(x.device)
         else:
-            import torch
-            with torch.cuda.stream(stream):  # the allocator then knows the memory's stream
-                out = MxMatrix.empty(rows, k, format, x.device)
-    elif out.rows != rows or out.k != k or out.format != format or out.device != x.get_device():
+            on = torch.cuda.ExternalStream(stream, x.device) if isinstance(stream, int) and stream else stream
+        with torch.cuda.stream(on or torch.cuda.default_stream(x.device)):  # the allocator then knows the memory's stream
+            out = MxMatrix.empty(rows, k, format, x.device)
+    to = out._key
+    if to[0] != rows or to[1] != k or to[2] != format or to[4] != x.get_device():
         raise ValueError("mx_quantize: out has another size, format or device")
     st = (_bound or _bind()).gz_mx_quantize(x.data_ptr(), api._torch_dtype_code(x.dtype), layout,
                                             strides[0] if shape[0] > 1 else 0, rows, k, format, multiplier, out._codes_ptr,
-                                            out.pitch, out._scales_ptr, out.device, _stream_handle(stream))
+                                            to[3], out._scales_ptr, to[4], _stream_handle(stream))
     if st != GZ_OK:
         raise GzError(st, "gz_mx_quantize")
     return out
@@ -195,11 +203,12 @@ def mx_dequantize(q: MxMatrix, out, layout=ROW_MAJOR, multiplier=1.0, stream=Non
     if len(shape) != 2 or not out.is_cuda or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
         _refuse_matrix(out, "mx_dequantize")
     rows, k = shape if layout == ROW_MAJOR else (shape[1], shape[0])
-    if q.rows != rows or q.k != k or q.device != out.get_device():
+    q_rows, q_k, format, pitch, device = q._key
+    if q_rows != rows or q_k != k or device != out.get_device():
         raise ValueError("mx_dequantize: out has another size or device")
-    st = (_bound or _bind()).gz_mx_dequantize(q._codes_ptr, q.pitch, q._scales_ptr, q.format, rows, k, multiplier,
+    st = (_bound or _bind()).gz_mx_dequantize(q._codes_ptr, pitch, q._scales_ptr, format, rows, k, multiplier,
                                               out.data_ptr(), api._torch_dtype_code(out.dtype), layout,
-                                              strides[0] if shape[0] > 1 else 0, q.device, _stream_handle(stream))
+                                              strides[0] if shape[0] > 1 else 0, device, _stream_handle(stream))
     if st != GZ_OK:
         raise GzError(st, "gz_mx_dequantize")
     return out

@@ -17,7 +17,8 @@
  * and stands for code * scale (* a multiplier the caller keeps, see below).
  *
  * Codes and scales must be 16-byte aligned.  Extents are positive (an empty matrix is refused, as
- * everywhere in this library).  Calls that overlap on the GPU may share inputs and plans freely: no
+ * everywhere in this library).  Outputs must not overlap inputs (D and C may be the same matrix; equal
+ * addresses of others are refused).  Calls that overlap on the GPU may share inputs and plans freely: no
  * entry point below keeps a workspace or counters between calls (a plan's status words apart). */
 #ifndef GEMMZOO_MICROSCALE_H
 #define GEMMZOO_MICROSCALE_H
@@ -109,7 +110,7 @@ GZ_API gz_status gz_mx_plan_destroy(gz_mx_plan* plan);
 GZ_API gz_status gz_mx_plan_info_get(const gz_mx_plan* plan, gz_mx_plan_info* info);
 
 /* D = act(alpha * row_scale[i] * col_scale[j] * (A B^T)[i][j] + beta * C + bias[j]), fp32 accumulation
- * and epilogue.  c may be NULL when *beta == 0 and may be d; ep may be NULL.  alpha, beta: host floats. */
+ * and epilogue.  c may be NULL when *beta == 0 and may be d (then with ldc == ldd); ep may be NULL.  alpha, beta: host floats. */
 GZ_API gz_status gz_mx_gemm_run(gz_mx_plan* plan, const void* a, const void* a_scales, const void* b,
                                 const void* b_scales, const void* c, void* d, const float* alpha, const float* beta,
                                 const gz_epilogue* ep, void* stream);

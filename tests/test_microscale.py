@@ -716,3 +716,52 @@ def test_withheld_signal_times_out_and_context_survives(config, m, split):
     assert plan.device_status()[0] == api.GZ_OK
     gz.MxGemm(m, n, k, FP4, torch.float32, config=config, split=split)(a, b, None, d, 1.0, 0.0)
     assert np.array_equal(d.cpu().double().numpy(), av @ bv.T)
+
+
+def test_in_place_conversions_are_refused():
+    L = ms._bind()
+    for src, codes, scales in ((4096, 4096, 8192), (4096, 8192, 4096), (4096, 8192, 8192)):
+        assert L.gz_mx_quantize(src, gz.DT_BF16, 0, 0, 4, 64, FP4, 1.0, codes, 0, scales, 0, None) == api.GZ_ERR_INVALID_ARG
+        assert L.gz_mx_dequantize(codes, 0, scales, FP4, 4, 64, 1.0, src, gz.DT_BF16, 0, 0, 0, None) == api.GZ_ERR_INVALID_ARG
+
+
+@gpu
+def test_overlapping_rows_of_codes_and_outputs_over_inputs_are_refused():
+    x = torch.randn(8, 64, device="cuda")
+    q = gz.mx_quantize(x, FP4)
+    for codes in (q.codes[:1].expand(8, 32), torch.zeros(160, dtype=torch.uint8, device="cuda").as_strided((8, 32), (16, 1))):
+        with pytest.raises(ValueError):
+            gz.MxMatrix(codes, q.scales, 8, 64, FP4)
+    with pytest.raises(AttributeError):
+        q.codes = q.codes.clone()
+    wide = torch.zeros(8, 16, device="cuda")
+    plan, mixed = gz.MxGemm(8, 8, 64, FP4, torch.float32), gz.MxGemm(8, 8, 64, FP4, torch.float32, ldc=16)
+    d = wide[:, :8].contiguous()
+    with pytest.raises(gz.GzError):
+        plan(q, q, None, q.codes.data_ptr(), 1.0, 0.0)
+    with pytest.raises(gz.GzError):
+        mixed(q, q, d.data_ptr(), d, 1.0, 1.0)
+    mixed(q, q, wide[:, :8], d, 1.0, 1.0)
+    chain = gz.MxGated(8, 64, 64, FP4, FP4)
+    out = gz.MxMatrix.empty(8, 64, FP4)
+    up = gz.mx_quantize(torch.randn(64, 64, device="cuda"), FP4)
+    chain(q, up, up, out)
+    for bad in (q, gz.MxMatrix(out.codes, q.scales, 8, 64, FP4), gz.MxMatrix(q.codes, out.scales, 8, 64, FP4)):
+        with pytest.raises(gz.GzError):
+            chain(q, up, up, bad)
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_new_matrices_belong_to_the_stream_that_writes_them():
+    """What mx_quantize allocates is freed in the order of the stream it was given, not of the current one."""
+    x = torch.randn(256, 1024, device="cuda")
+    want = gz.mx_quantize(x, NV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (side, side.cuda_stream, None, 0):
+        q = gz.mx_quantize(x, NV, stream=stream)
+        with torch.cuda.stream(side):
+            r = gz.mx_quantize(x, NV, stream=stream)
+        torch.cuda.synchronize()
+        assert torch.equal(q.codes, want.codes) and torch.equal(r.codes, want.codes) and torch.equal(r.scales, want.scales)
