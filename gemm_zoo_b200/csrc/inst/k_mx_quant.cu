@@ -48,8 +48,8 @@ cudaError_t quantize(bool cols, const gz::mx::QuantParams& p, cudaStream_t strea
   const int64_t padded = (p.rows + 127) / 128 * 128;  // the scale array's rows
   if (!cols) return launch_rows(gz::mx::quantize_rows_kernel<T, NV>, p, padded, p.groups * (NV ? 4 : 8), NV ? 4 : 8, stream);
   using Tile = gz::mx::ColTile<T>;
-  return launch(gz::mx::quantize_cols_kernel<T, NV>, p, grid_of(padded / Tile::ROWS, (p.k + gz::mx::COL_K - 1) / gz::mx::COL_K),
-                Tile::THREADS, stream);
+  return launch(p.vec == 32u ? gz::mx::quantize_cols_kernel<T, NV, true> : gz::mx::quantize_cols_kernel<T, NV, false>, p,
+                grid_of(padded / Tile::ROWS, (p.k + gz::mx::COL_K - 1) / gz::mx::COL_K), Tile::THREADS, stream);
 }
 template <typename T, bool NV>
 cudaError_t dequantize(bool cols, const gz::mx::QuantParams& p, cudaStream_t stream) {

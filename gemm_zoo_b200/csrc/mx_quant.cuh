@@ -49,7 +49,8 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // 32 bytes at a 32-byte aligned address.  What is quantised is read once and what is decoded written once, so
-// both may leave the L2 first: quantise and decode in turn 16384 x 4096 bf16 57.7 -> 52.3 us.
+// both may leave the L2 first: quantise and decode in turn 16384 x 4096 bf16 57.7 -> 53.4 us; 14336 x 4096 fp32
+// with K strided 113 -> 96 (16-byte accesses with the same hint: 101).
 __device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8]) {
   asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
@@ -205,7 +206,9 @@ struct ColTile {
   static __device__ __forceinline__ int at(int k, int row) { return k * PITCH + (k >> 4) * 8 + row; }
 };
 
-template <typename T, bool NV>
+// WIDE: every line is 32-byte aligned, and whole tiles are read 32 bytes at a time.  A kernel of its own, because
+// all three ways of reading in one need more registers (14340 x 4096 fp32, e4m3 blocks: 53 -> 61 us).
+template <typename T, bool NV, bool WIDE>
 __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(const QuantParams p) {
   using Tile = ColTile<T>;
   __shared__ __align__(16) T tile[Tile::ELEMS];
@@ -220,7 +223,13 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
   const int line = threadIdx.x / Tile::PER_LINE, piece = (threadIdx.x % Tile::PER_LINE) * VEC;
   constexpr int STEP = Tile::THREADS / Tile::PER_LINE;  // lines per pass
   uint4 w[LINES];
-  if (p.vec && k0 + COL_K <= p.k && row0 + Tile::ROWS <= p.rows) {
+  const bool inside = k0 + COL_K <= p.k && row0 + Tile::ROWS <= p.rows;
+  const int line2 = threadIdx.x / (Tile::PER_LINE / 2), piece2 = (threadIdx.x % (Tile::PER_LINE / 2)) * 2 * VEC;
+  if (WIDE && inside) {
+#pragma unroll
+    for (int l = 0; l < LINES / 2; ++l)
+      load32(src + static_cast<int64_t>(l * 2 * STEP + line2) * p.ld + piece2, *reinterpret_cast<uint32_t(*)[8]>(&w[2 * l]));
+  } else if (!WIDE && p.vec && inside) {
 #pragma unroll
     for (int l = 0; l < LINES; ++l)
       w[l] = __ldcs(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(l * STEP + line) * p.ld + piece));
@@ -229,7 +238,7 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
     for (int l = 0; l < LINES; ++l) {
       w[l] = make_uint4(0u, 0u, 0u, 0u);
       const int kk = l * STEP + line;
-      if (p.vec && k0 + kk < p.k) {
+      if ((WIDE || p.vec) && k0 + kk < p.k) {
         const T* s = src + static_cast<int64_t>(kk) * p.ld + piece;
         if (row0 + piece + VEC <= p.rows) {
           w[l] = *reinterpret_cast<const uint4*>(s);
@@ -242,7 +251,15 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
       }
     }
   }
-  if (p.vec) {
+  if (WIDE && inside) {
+    const bool swap = (threadIdx.x & 4u) != 0u;  // every other four lanes begin with their second piece: other banks
+#pragma unroll
+    for (int l = 0; l < LINES / 2; ++l) {
+      T* const to = &tile[Tile::at(l * 2 * STEP + line2, piece2)];
+      *reinterpret_cast<uint4*>(to + (swap ? VEC : 0)) = swap ? w[2 * l + 1] : w[2 * l];
+      *reinterpret_cast<uint4*>(to + (swap ? 0 : VEC)) = swap ? w[2 * l] : w[2 * l + 1];
+    }
+  } else if (WIDE || p.vec) {
 #pragma unroll
     for (int l = 0; l < LINES; ++l) *reinterpret_cast<uint4*>(&tile[Tile::at(l * STEP + line, piece)]) = w[l];
   } else {
@@ -410,8 +427,22 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(co
     }
     return;
   }
-  const int line = threadIdx.x / Tile::PER_LINE, piece = (threadIdx.x % Tile::PER_LINE) * VEC;
   constexpr int STEP = Tile::THREADS / Tile::PER_LINE;
+  if (p.vec == 32u && k0 + COL_K <= p.k && row0 + Tile::ROWS <= p.rows) {  // as in quantize_cols_kernel
+    const int line2 = threadIdx.x / (Tile::PER_LINE / 2), piece2 = (threadIdx.x % (Tile::PER_LINE / 2)) * 2 * VEC;
+    const bool swap = (threadIdx.x & 4u) != 0u;
+#pragma unroll
+    for (int l = 0; l < COL_K / STEP / 2; ++l) {
+      const int kk = l * 2 * STEP + line2;
+      const uint4* e = reinterpret_cast<const uint4*>(&tile[Tile::at(kk, piece2)]);
+      const uint4 a = e[swap ? 1 : 0], b = e[swap ? 0 : 1];
+      const uint4 lo = swap ? b : a, hi = swap ? a : b;
+      const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      store32(dst + static_cast<int64_t>(kk) * p.ld + piece2, words);
+    }
+    return;
+  }
+  const int line = threadIdx.x / Tile::PER_LINE, piece = (threadIdx.x % Tile::PER_LINE) * VEC;
 #pragma unroll
   for (int l = 0; l < COL_K / STEP; ++l) {
     const int kk = l * STEP + line;
