@@ -110,6 +110,7 @@ struct MxCfg {
   static constexpr int SLOT_COLS = 16;
   static constexpr int TMEM_COLS = ACC_COLS + 64 <= 128 ? 128 : ACC_COLS + 64 <= 256 ? 256 : 512;
   static_assert(ACC_COLS % 16 == 0 && ACC_COLS + 64 <= TMEM_COLS && (!SWAP || TMEM_COLS <= 256), "tensor memory");
+  // (a row tile's B scales have to start at a whole scale tile: 128 rows)
   static_assert(SWAP ? (BN % 16 == 0 && CTAS == 1) : (BN == 256 || (BN == 128 && !GATED)), "tile shapes");
   static_assert(STAGE_BYTES % 1024 == 0 && STAGES >= 2, "ring");
   static_assert(MB * BN * 128 * 4 <= RING_BYTES, "partial sums meet in the ring");
@@ -495,6 +496,10 @@ __device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* t
   detail::mx_store_box(p, tm_d, stg, lane, f, row0, col0, turn);
 }
 
+// What it measured (CUDA-graph replays over rotating operands, one B200): 8192^3, e8m0, bf16 out: 188 to 195 us, 5.6 to
+// 5.8 PFLOP/s, the tensor pipe busy 81 % of the cycles at a clock that the power limit holds at 1.3 to 1.55 GHz.  Two thousand
+// rows x 14336 x 4096, e4m3: product 51, + C 58, gated 93 us: tensor-bound, with the last wave of tiles partly empty.
+// One row x 14336 x 4096: product 9.5 us, gated 13.5 us: B at the copy rate (5.0, 9.5) and about 4 us of a launch's two ends.
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, Cfg::PER_SM)
 mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {

@@ -1,7 +1,12 @@
 // Quantisation to the microscaled 4-bit formats and its inverse (include/gemmzoo/microscale.h).
 //
 // Both are one pass over memory: a block's scale needs its largest magnitude, which a thread (or
-// two neighbouring ones) holds in registers, so a value is read once and its code written once.
+// two neighbouring ones) holds in registers, so a value is read once and its code written once.  HBM bounds
+// them from some 10 MB on.  Measured as CUDA-graph replays (quantise, decode; share of the measured copy rate):
+//   16384 x 4096 bf16, e8m0                28.7 us (90 %), 28.4 us (91 %)
+//   14336 x 4096 fp32, e4m3, K contiguous  41.7 us (98 %), 40.6 us (100 %)
+//   14336 x 4096 fp32, e4m3, K strided     46.3 us (88 %), 45.6 us (90 %)
+//   14336 x 4096 bf16, e4m3, K strided     34.3 us (67 %), 29.8 us (77 %): the quantiser nears its issue rate
 #ifndef GZ_MX_QUANT_CUH
 #define GZ_MX_QUANT_CUH
 

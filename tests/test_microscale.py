@@ -765,3 +765,34 @@ def test_new_matrices_belong_to_the_stream_that_writes_them():
             r = gz.mx_quantize(x, NV, stream=stream)
         torch.cuda.synchronize()
         assert torch.equal(q.codes, want.codes) and torch.equal(r.codes, want.codes) and torch.equal(r.scales, want.scales)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("layout", [gz.ROW_MAJOR, gz.COL_MAJOR])
+def test_quantise_and_decode_beyond_32_bit_offsets(fmt, layout):
+    """2.6e9 values: the last rows come out as those rows alone do."""
+    rows, k, tail = 40000, 65536, 64  # (the tail starts at a whole row group of the scales)
+    shape = (rows, k) if layout == gz.ROW_MAJOR else (k, rows)
+    x = torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_()
+    last = (x[-tail:] if layout == gz.ROW_MAJOR else x[:, -tail:]).contiguous()
+    q, w = gz.mx_quantize(x, fmt, layout=layout), gz.mx_quantize(last, fmt, layout=layout)
+    assert (rows - tail) % 128 == 0
+    assert torch.equal(q.codes[-tail:], w.codes) and torch.equal(q.scales[-w.scales.numel():], w.scales)
+    back = gz.mx_dequantize(q, x, layout=layout)
+    assert torch.equal((back[-tail:] if layout == gz.ROW_MAJOR else back[:, -tail:]), gz.mx_dequantize(w, last, layout=layout))
+
+
+@gpu
+@pytest.mark.parametrize("config", [gz.MX_CFG_PAIR, gz.MX_CFG_SINGLE_N128])
+def test_products_beyond_32_bit_offsets(config):
+    """A result of 2.6e9 values, C and D: the last rows come out as those rows alone do."""
+    m, n, k, tail = 40000, 65536, 64, 64
+    (a, _), (b, _) = _mx(m, k, NV, 1, True), _mx(n, k, NV, 2, True)
+    d = torch.ones(m, n, dtype=torch.float16, device="cuda")
+    gz.MxGemm(m, n, k, NV, torch.float16, config=config)(a, b, d, d, 1.0 / 64, 2.0)
+    blocks = -(-k // 64) * 512
+    rest = gz.MxMatrix(a.codes[-tail:], a.scales[(m - tail) // 128 * blocks:], tail, k, NV)
+    want = torch.ones(tail, n, dtype=torch.float16, device="cuda")
+    gz.MxGemm(tail, n, k, NV, torch.float16)(rest, b, want, want, 1.0 / 64, 2.0)
+    assert (m - tail) % 128 == 0 and torch.equal(d[-tail:], want)
