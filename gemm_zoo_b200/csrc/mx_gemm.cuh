@@ -237,15 +237,17 @@ __device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], 
 }
 
 // 32 rows x 32 columns (lane = row) to the output through the warp's 4 KB of staging: a TMA store of a
-// swizzled box, or, where TMA cannot describe D, whole row pieces with plain stores.  `turn` alternates
-// the two halves of the staging for 16-bit outputs.
+// swizzled box, or, where TMA cannot describe D, whole row pieces with plain stores.  The latter also for a last
+// box whose rows end inside 16 bytes: a TMA store ends there at the next multiple of 16 bytes and would write to
+// what lies beside D.  `turn` alternates the two halves of the staging for 16-bit outputs.
 __device__ __forceinline__ void mx_store_box(const MxParams& p, const void* tm_d, uint32_t stg, uint32_t lane,
                                              const float (&f)[32], uint32_t row0, uint32_t col0, uint32_t& turn) {
   const bool wide = p.out_type == 2u;
   const uint32_t box = wide ? stg : stg + (turn & 1u) * 2048u;
+  const bool tma = p.out_tma && (col0 + 32u <= p.n || (p.n & (wide ? 3u : 7u)) == 0u);
   if (p.out_tma) {
     if (lane == 0) {
-      if (wide) ptx::bulk_wait_group_read<0>();
+      if (wide || !tma) ptx::bulk_wait_group_read<0>();  // (a box without a group of its own: the next may wait for one only)
       else ptx::bulk_wait_group_read<1>();
     }
   }
@@ -271,7 +273,7 @@ __device__ __forceinline__ void mx_store_box(const MxParams& p, const void* tm_d
                    "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
                    : "memory");
   }
-  if (p.out_tma) {
+  if (tma) {
     ptx::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {

@@ -796,3 +796,27 @@ def test_products_beyond_32_bit_offsets(config):
     want = torch.ones(tail, n, dtype=torch.float16, device="cuda")
     gz.MxGemm(tail, n, k, NV, torch.float16)(rest, b, want, want, 1.0 / 64, 2.0)
     assert (m - tail) % 128 == 0 and torch.equal(d[-tail:], want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("config,split", [(gz.MX_CFG_PAIR, 1), (gz.MX_CFG_SINGLE, 2), (gz.MX_CFG_PAIR_N128, 1), (gz.MX_CFG_SINGLE_N128, 4), (gz.MX_CFG_SWAP_M64, 1)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_nothing_beside_the_result_is_written(dtype, config, split, gated):
+    """Results whose rows end anywhere within 16 bytes, in a matrix whose rows start at multiples of 16 bytes."""
+    if gated and config in (gz.MX_CFG_PAIR_N128, gz.MX_CFG_SINGLE_N128):
+        return
+    m, k, step = 60, 1100, 16 // torch.empty(0, dtype=dtype).element_size()
+    (a, av) = _mx(m, k, FP4, 1, True)
+    for n in (256 + step, 257, 258, 259, 385, 387):
+        (b, bv), (u, uv) = _mx(n, k, FP4, n, True), _mx(n, k, FP4, n + 1000, True)
+        full, d = _out(m, n, -(-n // step) * step + step, dtype)
+        if gated:
+            gz.MxGated(m, n, k, FP4, dtype, activation=gz.ACT_RELU, ldd=full.stride(0), config=config, split=split)(a, b, u, d[:, :n])
+            want = np.maximum(av @ bv.T, 0) * (av @ uv.T)
+        else:
+            gz.MxGemm(m, n, k, FP4, dtype, ldd=full.stride(0), config=config, split=split)(a, b, None, d[:, :n], 1.0, 0.0)
+            want = av @ bv.T
+        torch.cuda.synchronize()
+        assert torch.equal(d[:, :n].cpu(), torch.from_numpy(want).float().to(dtype))
+        assert _guards_intact(full, m, n)
