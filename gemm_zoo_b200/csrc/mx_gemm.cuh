@@ -40,6 +40,8 @@
 #ifndef GZ_MX_GEMM_CUH
 #define GZ_MX_GEMM_CUH
 
+#include <type_traits>
+
 #include "mx_format.cuh"
 #include "sm100_gemm.cuh"
 
@@ -191,9 +193,33 @@ __device__ __forceinline__ void mx_load_c_words(const MxParams& p, uint32_t row,
   }
 }
 
-// The optional terms on 32 columns of one row (row tiles); w: the words that mx_load_c_words read.
-__device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], const uint32_t (&w)[32], uint32_t row,
-                                             uint32_t col0, uint32_t lane) {
+// The same for a C whose rows cannot be read 16 bytes at a time: the warp takes one row after the other, a lane one
+// column, and mx_row_terms turns the box (a lane's own row in single values measured 1265 us for 8192 x 16383 fp16 at
+// k = 64, this 419).
+__device__ __forceinline__ void mx_load_c_rows(const MxParams& p, uint32_t row0, uint32_t col0, uint32_t lane, uint32_t (&w)[32]) {
+  if (row0 >= p.m || col0 >= p.n) return;
+  const uint32_t rows = col0 + lane < p.n ? p.m - row0 : 0u;  // that this lane has a column of
+  const int64_t at = static_cast<int64_t>(row0) * p.ldc + col0 + lane;
+  if (p.out_type == 2u) {
+    const uint32_t* c = static_cast<const uint32_t*>(p.c) + at;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) w[r] = static_cast<uint32_t>(r) < rows ? c[r * p.ldc] : 0u;
+  } else {
+    const uint16_t* c = static_cast<const uint16_t*>(p.c) + at;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) w[r] = static_cast<uint32_t>(r) < rows ? c[r * p.ldc] : 0u;
+  }
+}
+template <bool BY_ROWS>
+__device__ __forceinline__ void mx_load_c_box(const MxParams& p, uint32_t row0, uint32_t col0, uint32_t lane, uint32_t (&w)[32]) {
+  if constexpr (BY_ROWS) mx_load_c_rows(p, row0, col0, lane, w);
+  else mx_load_c_words(p, row0 + lane, col0, w);
+}
+
+// The optional terms on 32 columns of one row (row tiles); w: the words that mx_load_c_box read.
+template <bool BY_ROWS>
+__device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], const uint32_t (&w)[32], uint32_t stg,
+                                             uint32_t row, uint32_t col0, uint32_t lane) {
   const bool row_ok = row < p.m;
   const uint32_t ncols = p.n - col0 < 32u ? p.n - col0 : 32u;
   const bool col_ok = lane < ncols;
@@ -207,7 +233,25 @@ __device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], 
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] *= __shfl_sync(0xFFFFFFFFu, mine, i);
   }
-  if (p.beta != 0.0f && row_ok) {
+  if constexpr (BY_ROWS) {
+    // turned in the staging, whose rows are rotated so that neither side meets a bank twice
+    if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (uint32_t r = 0; r < 32; ++r) {
+      const float c = p.out_type == 2u   ? __uint_as_float(w[r])
+                      : p.out_type == 0u ? unpack2<__half>(w[r]).x
+                                         : unpack2<__nv_bfloat16>(w[r]).x;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(stg + r * 128u + (((lane + r) & 31u) << 2)), "f"(c) : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 32; ++i) {
+      float c;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c) : "r"(stg + lane * 128u + (((i + lane) & 31u) << 2)) : "memory");
+      f[i] = fmaf(p.beta, c, f[i]);
+    }
+  } else if (p.beta != 0.0f && row_ok) {
     if (mx_c_vectors(p, row, col0)) {
       if (p.out_type == 2u) {
 #pragma unroll
@@ -282,20 +326,30 @@ __device__ __forceinline__ void mx_store_box(const MxParams& p, const void* tm_d
     }
   } else {
     __syncwarp();
-    const uint32_t rows = p.m - row0 < 32u ? p.m - row0 : 32u;
-    const bool ok = lane < p.n - col0;
-#pragma unroll 8
-    for (uint32_t r = 0; r < rows; ++r) {
-      const int64_t at = static_cast<int64_t>(row0 + r) * p.ldd + col0 + lane;
-      if (!ok || !GZ_MX_STORE_OK(p, row0 + r, col0 + lane, 1u, p.m, p.n)) continue;
-      if (wide) {
-        uint32_t v;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(box + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u) : "memory");
-        static_cast<uint32_t*>(p.d)[at] = v;
-      } else {
-        uint16_t v;
-        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(box + r * 64u + (((lane >> 3) ^ ((r >> 1) & 3u)) << 4) + (lane & 7u) * 2u) : "memory");
-        static_cast<uint16_t*>(p.d)[at] = v;
+    const uint32_t rows = lane < p.n - col0 ? p.m - row0 : 0u;  // that this lane has a column of
+    // Four values out of shared memory, then four stores: one after the other costs a latency per row.  8192 x 16383 fp16
+    // at k = 64: 1 / 4 / 8 at a time 248 / 214 / 192 us, but with 8 the aligned form with C, short of registers,
+    // goes from 58 to 66 us (2048 x 14336 x 4096 fp16).
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < 32u; r0 += 4u) {
+      const int64_t at = static_cast<int64_t>(row0 + r0) * p.ldd + col0 + lane;
+      uint32_t v[4];
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t r = r0 + e;
+        if (wide) {
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[e]) : "r"(box + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u) : "memory");
+        } else {
+          uint16_t h;
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(h) : "r"(box + r * 64u + (((lane >> 3) ^ ((r >> 1) & 3u)) << 4) + (lane & 7u) * 2u) : "memory");
+          v[e] = h;
+        }
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        if (r0 + e >= rows || !GZ_MX_STORE_OK(p, row0 + r0 + e, col0 + lane, 1u, p.m, p.n)) continue;
+        if (wide) static_cast<uint32_t*>(p.d)[at + e * p.ldd] = v[e];
+        else static_cast<uint16_t*>(p.d)[at + e * p.ldd] = static_cast<uint16_t>(v[e]);
       }
     }
     __syncwarp();
@@ -465,8 +519,8 @@ __device__ __forceinline__ void mx_clear_scale_row(const MxParams& p, uint32_t t
 }
 
 // 32 columns of one row (lane = row) of a row tile, from the sums x (gated: and y) to the output.  c holds
-// the words of C for these columns on entry and those for next_col0 on return.
-template <class Cfg>
+// the words of C for these columns on entry and those for next_col0 on return (C_ROWS: see mx_load_c_rows).
+template <class Cfg, bool C_ROWS>
 __device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* tm_d, uint32_t stg, uint32_t lane,
                                                 const uint32_t (&x)[32], const uint32_t (&y)[32], uint32_t (&c)[32],
                                                 uint32_t row0, uint32_t col0, uint32_t next_col0, uint32_t& turn) {
@@ -487,12 +541,12 @@ __device__ __forceinline__ void mx_finish_slice(const MxParams& p, const void* t
     if (row0 >= p.m || col0 >= p.n) return;
   } else {
     if (row0 >= p.m || col0 >= p.n) {
-      detail::mx_load_c_words(p, row0 + lane, next_col0, c);  // the first group of an even tile may lie outside
+      detail::mx_load_c_box<C_ROWS>(p, row0, next_col0, lane, c);  // the first group of an even tile may lie outside
       return;
     }
     if (p.epi_flags != 0u || p.beta != 0.0f || p.act != 0u) {
-      detail::mx_row_terms(p, f, c, row0 + lane, col0, lane);
-      detail::mx_load_c_words(p, row0 + lane, next_col0, c);
+      detail::mx_row_terms<C_ROWS>(p, f, c, stg, row0 + lane, col0, lane);
+      detail::mx_load_c_box<C_ROWS>(p, row0, next_col0, lane, c);
     }
   }
   detail::mx_store_box(p, tm_d, stg, lane, f, row0, col0, turn);
@@ -841,6 +895,9 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
       constexpr uint32_t TILE_COLS = GATED ? BN / 2u : BN;  // output columns
       constexpr uint32_t GROUPS = TILE_COLS / 64u;          // of 64; this warp's half of each is 32 wide
       uint32_t turn = 0;
+      // One of two copies runs: one loop for both ways of reading C costs the aligned one (2048 x 14336 x 4096 fp16: 57 -> 62 us).
+      auto finish_tiles = [&](auto by_rows) {
+      constexpr bool C_ROWS = decltype(by_rows)::value;
       if (p.split <= 1u) {
         const uint32_t release = ptx::mapa(acc_empty_bar, leader);
         uint32_t it = 0;
@@ -852,7 +909,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
           // the group that the next tile's accumulator overlaps comes first
           auto group_col = [&](uint32_t s) { return tile_col + ((it & 1u) ? s : (s + GROUPS - 1u) % GROUPS) * 64u; };
           uint32_t c[32];
-          if constexpr (!GATED) detail::mx_load_c_words(p, row0 + lane, group_col(0), c);
+          if constexpr (!GATED) detail::mx_load_c_box<C_ROWS>(p, row0, group_col(0), lane, c);
           if (!__all_sync(0xFFFFFFFFu, detail::wait(acc_full_bar, it & 1u, ab, WAIT_EPILOGUE_TMEM_FULL, t, 0))) break;
           ptx::tc_fence_after_sync();
           const uint32_t acc = lanes + (it & 1u) * Cfg::ACC_STRIDE;
@@ -868,7 +925,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
               __syncwarp();
               if (lane == 0) ptx::mbar_arrive_cluster(release);
             }
-            mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, c, row0, col0, s + 1u < GROUPS ? group_col(s + 1u) : p.n, turn);
+            mx_finish_slice<Cfg, C_ROWS>(p, &maps.d, stg, lane, x, y, c, row0, col0, s + 1u < GROUPS ? group_col(s + 1u) : p.n, turn);
           }
           // one release per tile, made above; the rest of this tile's columns are read before the next
           // tile's release, which is what the tile after that waits for
@@ -909,7 +966,7 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
             if ((sl & 1u) != half) continue;
             const uint32_t col0 = tn * TILE_COLS + sl * 32u;
             uint32_t x[32], y[32], c[32];
-            if constexpr (!GATED) detail::mx_load_c_words(p, row0 + lane, col0, c);
+            if constexpr (!GATED) detail::mx_load_c_box<C_ROWS>(p, row0, col0, lane, c);
             for (uint32_t q = 0; q < p.split; ++q) {
               const uint32_t peer = ptx::mapa(mine, CTAS == 2 ? q * 2u + rank : q) + sl * (8u * 2048u);
 #pragma unroll
@@ -923,10 +980,13 @@ mx_gemm_kernel(const __grid_constant__ MxMaps maps, const MxParams p) {
                   sum[i] = __float_as_uint(q == 0u ? v[i / 4][i % 4] : __uint_as_float(sum[i]) + v[i / 4][i % 4]);
               }
             }
-            mx_finish_slice<Cfg>(p, &maps.d, stg, lane, x, y, c, row0, col0, p.n, turn);
+            mx_finish_slice<Cfg, C_ROWS>(p, &maps.d, stg, lane, x, y, c, row0, col0, p.n, turn);
           }
         }
       }
+      };
+      if (!GATED && p.beta != 0.0f && !p.c_vec_ok) finish_tiles(std::integral_constant<bool, !GATED>{});
+      else finish_tiles(std::false_type{});
       if (p.out_tma && lane == 0) ptx::bulk_wait_group_read<0>();
     }
   }
