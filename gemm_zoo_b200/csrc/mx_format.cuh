@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "ptx.cuh"
+
 namespace gz {
 namespace mx {
 
@@ -28,9 +30,7 @@ __host__ __device__ __forceinline__ int64_t scale_word(int64_t r, int64_t g, int
 
 // max(|a|, |b|) that keeps a NaN.
 __device__ __forceinline__ float amax_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
-  return r;
+  return ptx::max_nan(fabsf(a), fabsf(b));
 }
 
 // A block's scale from the largest magnitude in it, and what turns its values into code units.

@@ -33,6 +33,13 @@ __device__ __forceinline__ bool elect_one() {
   return pred != 0;
 }
 
+// The larger of two numbers; a NaN if either is one (fmaxf returns the other number).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Index of the SM this thread runs on.
 __device__ __forceinline__ uint32_t smid() {
   uint32_t r;

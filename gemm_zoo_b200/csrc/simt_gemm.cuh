@@ -16,6 +16,8 @@
 
 #include <type_traits>
 
+#include "ptx.cuh"
+
 namespace gz {
 
 struct SimtParams {
@@ -72,7 +74,7 @@ __device__ __forceinline__ __nv_bfloat16 simt_from_f<__nv_bfloat16>(float v) {
 }
 __device__ __forceinline__ float simt_activate(float x, uint32_t act) {
   switch (act) {
-    case 1: return fmaxf(x, 0.0f);
+    case 1: return ptx::max_nan(x, 0.0f);
     case 2: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
     case 3: {
       const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);

@@ -409,7 +409,7 @@ __device__ __forceinline__ float erf_fast(float z) {
 
 __device__ __forceinline__ float activate(float x, uint32_t act) {
   switch (act) {
-    case 1: return fmaxf(x, 0.0f);
+    case 1: return ptx::max_nan(x, 0.0f);
     case 2: return 0.5f * x * (1.0f + erf_fast(x * 0.70710678118654752f));
     case 3: {
       // 0.5 x (1 + tanh u) with tanh u = 1 - 2 / (e^(2u) + 1), i.e. x (1 - 1 / (e^(2u) + 1)): one

@@ -207,7 +207,7 @@ GZ_API gz_status gz_gemm_run(gz_plan* plan, const void* a, const void* b, const 
  * (intel/test/utils.hpp:133-136). */
 typedef enum gz_activation {
   GZ_ACT_NONE = 0,
-  GZ_ACT_RELU = 1,
+  GZ_ACT_RELU = 1,      /* max(x, 0); a NaN stays a NaN, as in the others */
   GZ_ACT_GELU = 2,      /* 0.5 x (1 + erf(x / sqrt 2)) */
   GZ_ACT_GELU_TANH = 3, /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
   GZ_ACT_SILU = 4       /* x / (1 + exp(-x)) */
