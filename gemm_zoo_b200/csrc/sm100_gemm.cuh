@@ -1434,7 +1434,10 @@ sm100_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
               for (uint32_t box = 0; box * BOX_COLS < wcols; ++box) {
                 const uint32_t box_col = col_w + box * BOX_COLS;
                 if (box_col >= p.n) break;
-                if (p.epilogue_tma) {
+                // A TMA store whose rows end within 16 bytes writes zeros up to the next multiple of 16
+                // bytes, beside D: such a box (a row's last) is stored plainly.
+                const bool box_tma = p.epilogue_tma && (box_col + BOX_COLS <= p.n || p.n % (16 / sizeof(TOut)) == 0u);
+                if (box_tma) {
                   if (lane == 0) ptx::bulk_wait_group_read<0>();
                   __syncwarp();
                 }
@@ -1448,7 +1451,7 @@ sm100_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                   ptx::tmem_wait_ld();
                   const TOut* crow = cmat_b + static_cast<int64_t>(row) * p.ldc + col0;
                   detail::epilogue_math<TOut, ACC_INT>(x, p, crow, row_ok, ncols, row, col0);
-                  if (p.epilogue_tma) {
+                  if (box_tma) {
 #pragma unroll
                     for (int q = 0; q < WORDS / 4; ++q) {
                       const uint32_t j = static_cast<uint32_t>(sl * (WORDS / 4) + q);
@@ -1463,7 +1466,7 @@ sm100_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                       detail::store_direct<TOut>(x, drow, ncols, p.d_vec_ok != 0u);
                   }
                 }
-                if (p.epilogue_tma) {
+                if (box_tma) {
                   ptx::fence_proxy_async_smem();
                   __syncwarp();
                   if (lane == 0) {
