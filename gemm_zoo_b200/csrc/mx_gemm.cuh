@@ -224,12 +224,12 @@ __device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], 
   const uint32_t ncols = p.n - col0 < 32u ? p.n - col0 : 32u;
   const bool col_ok = lane < ncols;
   if (p.epi_flags & 2u) {
-    const float rs = row_ok ? __ldg(p.row_scale + row) : 1.0f;
+    const float rs = row_ok ? p.row_scale[row] : 1.0f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] *= rs;
   }
   if (p.epi_flags & 4u) {
-    const float mine = col_ok ? __ldg(p.col_scale + col0 + lane) : 1.0f;
+    const float mine = col_ok ? p.col_scale[col0 + lane] : 1.0f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] *= __shfl_sync(0xFFFFFFFFu, mine, i);
   }
@@ -273,7 +273,7 @@ __device__ __forceinline__ void mx_row_terms(const MxParams& p, float (&f)[32], 
     }
   }
   if (p.epi_flags & 1u) {
-    const float mine = col_ok ? __ldg(p.bias + col0 + lane) : 0.0f;
+    const float mine = col_ok ? p.bias[col0 + lane] : 0.0f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] += __shfl_sync(0xFFFFFFFFu, mine, i);
   }
@@ -421,7 +421,7 @@ __device__ __forceinline__ void mx_store_quantized_row(const MxParams& p, const 
 // Up to four columns of a row as fp32, and back (`n` of them exist).
 __device__ __forceinline__ void mx_load4(const float* v, uint32_t n, float (&f)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = static_cast<uint32_t>(i) < n ? __ldg(v + i) : 0.0f;
+  for (int i = 0; i < 4; ++i) f[i] = static_cast<uint32_t>(i) < n ? v[i] : 0.0f;
 }
 
 }  // namespace detail
@@ -447,7 +447,7 @@ __device__ __forceinline__ void mx_finish_row(const MxParams& p, float (&f)[4], 
   if constexpr (!Cfg::GATED) {
     float t[4];
     if (p.epi_flags & 2u) {
-      const float rs = __ldg(p.row_scale + row);
+      const float rs = p.row_scale[row];
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] *= rs;
     }

@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(const QuantParams 
     if (mine && row < p.rows) {
       codes[r] = *reinterpret_cast<const uint2*>(p.codes + row * p.pitch + k0 / 2);
       const int64_t block = k0 / BLOCK;
-      bytes[r] = __ldg(p.scales + scale_word(row, block >> 2, p.groups) + (block & 3));
+      bytes[r] = p.scales[scale_word(row, block >> 2, p.groups) + (block & 3)];
     }
   }
 #pragma unroll
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(co
     if (row < p.rows && kc < p.k) {
       codes[r] = *reinterpret_cast<const uint2*>(p.codes + row * p.pitch + kc / 2);
       const int64_t block = kc / BLOCK;
-      bytes[r] = __ldg(p.scales + scale_word(row, block >> 2, p.groups) + (block & 3));
+      bytes[r] = p.scales[scale_word(row, block >> 2, p.groups) + (block & 3)];
     }
   }
   float v[2][16];

@@ -101,7 +101,9 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v
 // Programmatic dependent launch.  launch_dependents: the next kernel of the stream (if it was
 // launched with programmatic serialization) may be scheduled once every CTA of this grid has said so
 // or exited.  wait: blocks until the kernels this grid depends on have completed and their memory
-// operations are visible; a no-op for a grid launched the ordinary way.
+// operations are visible; a no-op for a grid launched the ordinary way.  What those kernels may have written is read
+// with ordinary loads after the wait: the non-coherent path (__ldg) is for data that nothing writes while the grid is
+// resident, and a grid launched this way is resident while its predecessors still write.
 __device__ __forceinline__ void grid_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

@@ -425,12 +425,12 @@ __device__ __forceinline__ float activate(float x, uint32_t act) {
 // The optional terms around one element: epi_scale() takes alpha * acc, epi_finish() takes
 // alpha * rs * cs * acc + beta * c.
 __device__ __forceinline__ float epi_scale(const GemmParams& p, float f, uint32_t row, uint32_t col) {
-  if (p.row_scale) f *= __ldg(p.row_scale + row);
-  if (p.col_scale) f *= __ldg(p.col_scale + col);
+  if (p.row_scale) f *= p.row_scale[row];
+  if (p.col_scale) f *= p.col_scale[col];
   return f;
 }
 __device__ __forceinline__ float epi_finish(const GemmParams& p, float f, uint32_t col) {
-  if (p.bias) f += __ldg(p.bias + col);
+  if (p.bias) f += p.bias[col];
   return activate(f, p.act);
 }
 
@@ -503,8 +503,8 @@ __device__ __forceinline__ void epilogue_math(uint32_t (&v)[32], const GemmParam
     const uint32_t lane = ptx::lane_id();
     const bool col_ok = lane < ncols;
     if (epi) {
-      const float rs = (p.row_scale && row_ok) ? __ldg(p.row_scale + row) : 1.0f;
-      const float my_cs = (p.col_scale && col_ok) ? __ldg(p.col_scale + col0 + lane) : 1.0f;
+      const float rs = (p.row_scale && row_ok) ? p.row_scale[row] : 1.0f;
+      const float my_cs = (p.col_scale && col_ok) ? p.col_scale[col0 + lane] : 1.0f;
       if (p.row_scale) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] *= rs;
@@ -534,7 +534,7 @@ __device__ __forceinline__ void epilogue_math(uint32_t (&v)[32], const GemmParam
     }
     if (epi) {
       if (p.bias) {
-        const float my_bias = col_ok ? __ldg(p.bias + col0 + lane) : 0.0f;
+        const float my_bias = col_ok ? p.bias[col0 + lane] : 0.0f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] += __shfl_sync(0xFFFFFFFFu, my_bias, i);
       }
