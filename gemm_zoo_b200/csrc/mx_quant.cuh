@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
   ptx::grid_dependency_wait();
   int64_t row0, chunk;
   const bool mine = row_item(p, row0, chunk, ROWS_PER_THREAD) && chunk / PER_WORD < p.groups;
-  const uint32_t mask = __ballot_sync(__activemask(), mine);  // whole words: row_threads is a multiple of PER_WORD
+  // Every thread of the block gets here.  The lanes that go on are whole words of scales: row_threads is a multiple of PER_WORD.
+  const uint32_t mask = __ballot_sync(0xFFFFFFFFu, mine);
   if (!mine) return;
   const int64_t k0 = chunk * 16;
   uint32_t w[ROWS_PER_THREAD][WORDS];
