@@ -31,3 +31,97 @@ def test_rows_whose_words_end_inside_a_warp(fmt, dtype):
         for k in (words * word, words * word - 17):
             x = _values(5, k, dtype, 11)
             _check_quantised(x.double().numpy(), gz.mx_quantize(x.cuda(), fmt), fmt)
+
+
+# ------------------------------------------------------------------------------------------- shared K ranges
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("out", FORMATS)
+@pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_SWAP_M16, 1, 2), (gz.MX_CFG_SWAP_M16, 13, 4), (gz.MX_CFG_SWAP_M16, 16, 8),
+                                            (gz.MX_CFG_SWAP_M32, 21, 8), (gz.MX_CFG_SWAP_M32, 32, 2), (gz.MX_CFG_SWAP_M64, 50, 4),
+                                            (gz.MX_CFG_SWAP_M64, 64, 8), (gz.MX_CFG_SINGLE, 100, 2), (gz.MX_CFG_SINGLE, 130, 4),
+                                            (gz.MX_CFG_PAIR, 100, 2), (gz.MX_CFG_PAIR, 300, 2), (gz.MX_CFG_PAIR, 200, 4)])
+def test_quantised_gated_result_with_a_shared_k_range(fmt, out, config, m, split):
+    """Integer sums: codes and scales bit for bit, scale rows and blocks that do not exist 0, nothing else written."""
+    for n, k in [(1, 256 * split), (130, 256 * split + 17), (290, 256 * split + 900), (200, 4096)]:
+        (a, av), (g, gv), (u, uv) = _mx(m, k, fmt, 1, True), _mx(n, k, fmt, 2, True), _mx(n, k, fmt, 3, True)
+        sums = av @ gv.T, av @ uv.T
+        assert all(np.abs(s).max() < 2 ** 24 for s in sums)
+        # two roundings to fp32 at most: none of the scaled sums (powers of two), one of their product
+        want = (np.maximum(sums[0], 0) * 2.0 ** -8).astype(np.float32) * (sums[1] * 2.0 ** -8).astype(np.float32)
+        pitch, size = ms.code_pitch(n) + 16, ms.scale_bytes(out, m, n)
+        store = torch.full((m + 1, pitch), 0xEE, dtype=torch.uint8, device="cuda")
+        sc = torch.full((size + 64,), 0xEE, dtype=torch.uint8, device="cuda")
+        q = gz.MxMatrix(store[:m], sc, m, n, out)
+        plan = gz.MxGated(m, n, k, fmt, out, activation=gz.ACT_RELU, ldd=pitch, config=config, split=split, wait_limit_ns=200_000_000)
+        assert plan.info().split == split
+        plan(a, g, u, q, 2.0 ** -8, 2.0 ** -8, 2.0 ** -3)
+        assert plan.device_status()[0] == 0
+        _check_quantised(want.astype(np.float64) * 2.0 ** -3, q, out)
+        assert bool((store[:m, ms.code_pitch(n):] == 0xEE).all()) and bool((store[m] == 0xEE).all()) and bool((sc[size:] == 0xEE).all())
+
+
+SHARED = [(gz.MX_CFG_PAIR, 300, 2), (gz.MX_CFG_PAIR, 100, 4), (gz.MX_CFG_SINGLE, 200, 2), (gz.MX_CFG_SINGLE, 130, 8),
+          (gz.MX_CFG_PAIR_N128, 300, 2), (gz.MX_CFG_PAIR_N128, 520, 4), (gz.MX_CFG_SINGLE_N128, 130, 2), (gz.MX_CFG_SINGLE_N128, 100, 4),
+          (gz.MX_CFG_SWAP_M16, 9, 8), (gz.MX_CFG_SWAP_M32, 20, 2), (gz.MX_CFG_SWAP_M64, 64, 4)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("config,m,split", SHARED)
+def test_epilogue_terms_with_a_shared_k_range(dtype, config, m, split):
+    """C apart from D and in place, rows of C and D aligned and not, bias, row and column scales, ReLU.  Integers and powers
+    of two: every fp32 value is exact, so results are compared bit for bit after the one rounding to the output type."""
+    step = 16 // torch.empty(0, dtype=dtype).element_size()
+    for n, k, odd in [(264, 256 * split, 0), (261, 256 * split + 800, 3), (520, 256 * split + 15, step)]:
+        rng = np.random.default_rng([m, n, split])
+        (a, av), (b, bv) = _mx(m, k, NV, 4, True), _mx(n, k, NV, 5, True)
+        acc = av @ bv.T
+        c = rng.integers(-64, 65, (m, n)).astype(np.float64)
+        bias = rng.integers(-64, 65, n).astype(np.float32)
+        rs, cs = (2.0 ** rng.integers(-3, 2, r).astype(np.float32) for r in (m, n))
+        ldd = -(-n // step) * step + odd
+        for beta, terms, inplace in [(0.0, True, False), (-2.0, False, True), (-2.0, False, False), (3.0, True, True), (3.0, True, False)]:
+            full, d = _out(m, n, ldd, dtype)
+            cd = torch.from_numpy(c).to(dtype)
+            if inplace:
+                d[:, :n] = cd.cuda()
+                cc = d
+            else:
+                cc = torch.nn.functional.pad(cd, (0, odd)).cuda()
+            plan = gz.MxGemm(m, n, k, NV, dtype, ldc=cc.stride(0), ldd=ldd, config=config, split=split, wait_limit_ns=200_000_000)
+            assert plan.info().split == split
+            kw = dict(bias=torch.from_numpy(bias).cuda(), row_scale=torch.from_numpy(rs).cuda(), col_scale=torch.from_numpy(cs).cuda(),
+                      activation=gz.ACT_RELU) if terms else {}
+            plan(a, b, cc[:, :n] if beta else None, d[:, :n], 0.5, beta, **kw)
+            assert plan.device_status()[0] == 0
+            want = 0.5 * acc * (np.outer(rs.astype(np.float64), cs) if terms else 1.0) + beta * c + (bias if terms else 0.0)
+            assert np.abs(want).max() * 2.0 ** 6 < 2 ** 24  # in units of 2^-6, what the scales divide by
+            if terms:
+                want = np.maximum(want, 0)
+            assert torch.equal(d[:, :n].cpu(), torch.from_numpy(want).float().to(dtype)), (n, k, beta, terms, inplace)
+            assert _guards_intact(full, m, n)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 4096), (64, 512, 4096), (200, 512, 8192)])
+def test_chosen_configurations_share_the_k_range(fmt, m, n, k):
+    """The sizes of decoding steps, with the tile and split that are chosen for them; quantised and plain results."""
+    (a, av), (g, gv), (u, uv) = _mx(m, k, fmt, 1, True), _mx(n, k, fmt, 2, True), _mx(n, k, fmt, 3, True)
+    sums = av @ gv.T, av @ uv.T
+    assert all(np.abs(s).max() < 2 ** 24 for s in sums)
+    want = (np.maximum(sums[0], 0) * 2.0 ** -8).astype(np.float32) * (sums[1] * 2.0 ** -8).astype(np.float32)
+    for out in (fmt, torch.float32):
+        plan = gz.MxGated(m, n, k, fmt, out, activation=gz.ACT_RELU)
+        assert plan.info().split > 1
+        d = gz.MxMatrix.empty(m, n, out) if out is fmt else torch.empty(m, n, device="cuda")
+        plan(a, g, u, d, 2.0 ** -8, 2.0 ** -8)
+        if out is fmt:
+            _check_quantised(want.astype(np.float64), d, fmt)
+        else:
+            assert np.array_equal(d.cpu().numpy(), want)
+    d = torch.empty(m, n, device="cuda")
+    plan = gz.MxGemm(m, n, k, fmt, torch.float32)
+    plan(a, g, None, d, 1.0, 0.0)
+    assert plan.info().split > 1 and np.array_equal(d.cpu().double().numpy(), sums[0])
