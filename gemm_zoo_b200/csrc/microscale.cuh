@@ -475,6 +475,7 @@ GZ_API gz_status gz_mx_gemm_run(gz_mx_plan* pl, const void* a, const void* a_sca
   if (ep) {
     if (ep->struct_size != sizeof(gz_epilogue) || ep->activation < GZ_ACT_NONE || ep->activation > GZ_ACT_SILU)
       return GZ_ERR_INVALID_ARG;
+    if (d == ep->bias || d == ep->row_scale || d == ep->col_scale) return GZ_ERR_INVALID_ARG;  // read while others write
     if (!mx_aligned(ep->bias, 4) || !mx_aligned(ep->row_scale, 4) || !mx_aligned(ep->col_scale, 4)) return GZ_ERR_MISALIGNED;
     p.epi_flags = (ep->bias ? 1u : 0u) | (ep->row_scale ? 2u : 0u) | (ep->col_scale ? 4u : 0u);
     p.act = (uint32_t)ep->activation;

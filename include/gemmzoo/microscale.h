@@ -17,8 +17,8 @@
  * and stands for code * scale (* a multiplier the caller keeps, see below).
  *
  * Codes and scales must be 16-byte aligned.  Extents are positive (an empty matrix is refused, as
- * everywhere in this library).  Outputs must not overlap inputs (D and C may be the same matrix; equal
- * addresses of others are refused).  Calls that overlap on the GPU may share inputs and plans freely: no
+ * everywhere in this library).  Outputs must not overlap inputs, the epilogue's vectors among them (D and C may
+ * be the same matrix; equal addresses of others are refused).  Calls that overlap on the GPU may share inputs and plans freely: no
  * entry point below keeps a workspace or counters between calls (a plan's status words apart). */
 #ifndef GEMMZOO_MICROSCALE_H
 #define GEMMZOO_MICROSCALE_H

@@ -125,3 +125,19 @@ def test_chosen_configurations_share_the_k_range(fmt, m, n, k):
     plan = gz.MxGemm(m, n, k, fmt, torch.float32)
     plan(a, g, None, d, 1.0, 0.0)
     assert plan.info().split > 1 and np.array_equal(d.cpu().double().numpy(), sums[0])
+
+
+# ------------------------------------------------------------------------------------------- aliases
+@gpu
+@pytest.mark.parametrize("config", [gz.MX_CFG_SWAP_M16, gz.MX_CFG_SINGLE_N128, gz.MX_CFG_PAIR])
+def test_a_result_in_place_of_an_epilogue_vector_is_refused(config):
+    a, b = gz.mx_quantize(torch.randn(1, 256, device="cuda"), NV), gz.mx_quantize(torch.randn(300, 256, device="cuda"), NV)
+    plan, d = gz.MxGemm(1, 300, 256, NV, torch.float32, config=config), torch.ones(1, 300, device="cuda")
+    for name, v in (("bias", d[0]), ("col_scale", d[0]), ("row_scale", d[0, :1])):
+        with pytest.raises(gz.GzError) as e:
+            plan(a, b, None, d, 1.0, 0.0, **{name: v})
+        assert e.value.status == api.GZ_ERR_INVALID_ARG
+    torch.cuda.synchronize()
+    assert bool((d == 1).all())
+    plan(a, b, None, d, 1.0, 0.0, bias=torch.zeros(300, device="cuda"))
+    torch.cuda.synchronize()
