@@ -372,6 +372,8 @@ GZ_API gz_status gz_mx_dequantize(const void* codes, int64_t pitch, const void* 
   DeviceGuard guard(device);
   if (!guard.ok()) return (st = mx_device_ok(device)) != GZ_OK ? st : GZ_ERR_CUDA;
   p.out = dst;
+  p.pre = !nv && std::fabs(multiplier) < 1.0f ? 0.25f : 1.0f;
+  p.multiplier = multiplier / p.pre;
   p.codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
   p.scales = const_cast<uint8_t*>(static_cast<const uint8_t*>(scales));
   if (!cuda_ok(gz::mx_launch_dequantize(dst_type, nv, cols, p, static_cast<cudaStream_t>(stream)), "kernel launch"))

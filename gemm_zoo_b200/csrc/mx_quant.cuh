@@ -34,6 +34,7 @@ struct QuantParams {
   uint32_t vec;   // bytes that an access to the values may have: 32, 16, or 0 (single values)
   uint32_t unit;  // multiplier == 1
   float multiplier;
+  float pre;  // decode: a power of two that the scale is multiplied by first (`multiplier` has been divided by it)
 };
 
 template <typename T>
@@ -312,7 +313,8 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) quantize_cols_kernel(cons
 }
 
 // Dequantising: code * scale is exact in fp32; the product with the multiplier is rounded once there and
-// once to T.
+// once to T.  (6 * 2^127 is beyond fp32, though not what a small multiplier makes of it: `pre` takes such scales down by
+// an exact 1/4.)
 template <typename T, bool NV>
 __global__ void __launch_bounds__(256) dequantize_rows_kernel(const QuantParams p) {
   extern __shared__ __align__(16) uint8_t row_buffer[];  // 256 x 16 values where single values are stored, else none
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(const QuantParams 
 #pragma unroll
   for (int r = 0; r < ROWS_PER_THREAD; ++r) {
     const int64_t row = row0 + r * p.block_rows;
-    const float s = scale_value<NV>(bytes[r]);
+    const float s = scale_value<NV>(bytes[r]) * p.pre;
     float v[16];
     unpack8(codes[r].x, *reinterpret_cast<float(*)[8]>(&v[0]));
     unpack8(codes[r].y, *reinterpret_cast<float(*)[8]>(&v[8]));
@@ -411,7 +413,7 @@ __global__ void __launch_bounds__(ColTile<T>::THREADS) dequantize_cols_kernel(co
   float v[2][16];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const float s = scale_value<NV>(bytes[r]);
+    const float s = scale_value<NV>(bytes[r]) * p.pre;
     unpack8(codes[r].x, *reinterpret_cast<float(*)[8]>(&v[r][0]));
     unpack8(codes[r].y, *reinterpret_cast<float(*)[8]>(&v[r][8]));
 #pragma unroll

@@ -141,3 +141,24 @@ def test_a_result_in_place_of_an_epilogue_vector_is_refused(config):
     assert bool((d == 1).all())
     plan(a, b, None, d, 1.0, 0.0, bias=torch.zeros(300, device="cuda"))
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------- decoding
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("layout", [gz.ROW_MAJOR, gz.COL_MAJOR])
+@pytest.mark.parametrize("multiplier", [1.0, -1.0, 2.0 ** -10, 0.3, -0.9999999, 1.7, 2.0 ** -140, -3e38, 1e-38])
+def test_every_code_of_every_scale_decodes_to_its_product(fmt, layout, multiplier):
+    """code * scale * multiplier, rounded once to fp32 and once to the type, to infinity only where the product is beyond it."""
+    size, count = orc.block(fmt), 256 if fmt == FP4 else 128
+    codes = np.tile(np.arange(16, dtype=np.uint8), (count, size // 16))
+    scales = np.arange(count, dtype=np.uint8)[:, None]
+    q = gz.MxMatrix(torch.from_numpy(orc.pack(codes)).cuda(), torch.from_numpy(orc.tile(scales)).cuda(), count, size, fmt)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = (orc.decode(codes, scales, fmt) * float(np.float32(multiplier))).astype(np.float32)  # 2 + 24 bits: exact in 64
+    for dtype in (torch.float32, torch.bfloat16):
+        y = torch.empty((count, size) if layout == gz.ROW_MAJOR else (size, count), dtype=dtype, device="cuda")
+        gz.mx_dequantize(q, y, layout=layout, multiplier=multiplier)
+        got = y.cpu() if layout == gz.ROW_MAJOR else y.cpu().t()
+        ref = torch.from_numpy(want).to(dtype)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got[~torch.isnan(got)], ref[~torch.isnan(ref)])
