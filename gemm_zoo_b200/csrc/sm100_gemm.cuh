@@ -392,8 +392,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-__device__ __forceinline__ float erf_fast(float z) {
-  const float az = fabsf(z);
+// The two factors of 1 - erf(|z|), a polynomial in t and exp(-z^2).
+__device__ __forceinline__ void erfc_factors(float az, float& poly_t, float& e) {
   // The correctly rounded reciprocal on purpose: with rcp_approx here the epilogue of a tile is
   // 40 % shorter, but the main loop that runs beside it loses 7 % (measured at bf16 2048x14336x4096
   // with bias + GELU: MMA issue 215 -> 271 clocks per K block, 1.069x the plain GEMM instead of
@@ -403,8 +403,14 @@ __device__ __forceinline__ float erf_fast(float z) {
   poly = fmaf(poly, t, 1.421413741f);
   poly = fmaf(poly, t, -0.284496736f);
   poly = fmaf(poly, t, 0.254829592f);
-  const float e = __expf(-az * az);
-  return copysignf(fmaf(-poly * t, e, 1.0f), z);
+  poly_t = poly * t;
+  e = __expf(-az * az);
+}
+
+__device__ __forceinline__ float erf_fast(float z) {
+  float poly_t, e;
+  erfc_factors(fabsf(z), poly_t, e);
+  return copysignf(fmaf(-poly_t, e, 1.0f), z);
 }
 
 __device__ __forceinline__ float activate(float x, uint32_t act) {

@@ -110,7 +110,12 @@ GZ_API gz_status gz_mx_plan_destroy(gz_mx_plan* plan);
 GZ_API gz_status gz_mx_plan_info_get(const gz_mx_plan* plan, gz_mx_plan_info* info);
 
 /* D = act(alpha * row_scale[i] * col_scale[j] * (A B^T)[i][j] + beta * C + bias[j]), fp32 accumulation
- * and epilogue.  c may be NULL when *beta == 0 and may be d (then with ldc == ldd); ep may be NULL.  alpha, beta: host floats. */
+ * and epilogue.  c may be NULL when *beta == 0 and may be d (then with ldc == ldd); ep may be NULL.  alpha,
+ * beta: host floats.
+ *
+ * Activations are within 5e-7 |x| of their exact value at the fp32 x they are given, at a result of normal
+ * size SiLU and the tanh GELU also within (6e-7 + 5e-7 |y|) of the result (e^y is their exponential) and the
+ * erf GELU within 1e-4 of it for x >= -3, 1e-3 for x >= -4.5 and 1e-2 for x >= -7.5. */
 GZ_API gz_status gz_mx_gemm_run(gz_mx_plan* plan, const void* a, const void* a_scales, const void* b,
                                 const void* b_scales, const void* c, void* d, const float* alpha, const float* beta,
                                 const gz_epilogue* ep, void* stream);

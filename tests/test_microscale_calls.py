@@ -162,3 +162,80 @@ def test_every_code_of_every_scale_decodes_to_its_product(fmt, layout, multiplie
         got = y.cpu() if layout == gz.ROW_MAJOR else y.cpu().t()
         ref = torch.from_numpy(want).to(dtype)
         assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got[~torch.isnan(got)], ref[~torch.isnan(ref)])
+
+
+# ------------------------------------------------------------------------------------------- activations
+def _activated(x, act, config, m):
+    """act of the values x: the bias of a product that is zero."""
+    n = x.numel()
+    a, b = gz.mx_quantize(torch.zeros(m, 64, device="cuda"), FP4), gz.mx_quantize(torch.zeros(n, 64, device="cuda"), FP4)
+    d = torch.empty(m, n, device="cuda")
+    gz.MxGemm(m, n, 64, FP4, torch.float32, config=config)(a, b, None, d, 1.0, 0.0, bias=x.cuda(), activation=ACTS[act])
+    d = d.cpu()
+    assert all(torch.equal(d[i], d[0]) for i in range(m)) or bool(torch.isnan(x).any())
+    return d[0].double().numpy()
+
+
+@gpu
+@pytest.mark.parametrize("config,m", [(gz.MX_CFG_SWAP_M16, 2), (gz.MX_CFG_PAIR, 130)])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_over_their_range(act, config, m):
+    """The absolute bound (5e-7 |x|) and the relative one where the result is small.
+
+    With u = 2^-24 and __expf good to (2 + 1.173 |y|) * 2u: e^y is off by at most |y| * (y's own relative error, 6u for
+    the tanh form's argument, 0 for SiLU's, 1.173 * 2u for __expf) + 4u, relative; a sigmoid s = 1 / (1 + e^y) by (1 - s)
+    times that, + 4u for the sum, the approximate reciprocal and the product: 5e-7 |y| + 6e-7 relative, and, as
+    s (1 - s) |y| < 0.23 and s (1 - s) <= 1/4, 4e-7 absolute.  erfc(z) = p(t) t e^(-z^2) is good to 1.5e-7 by its
+    source; its factors' roundings are at most 5u + 7u z^2 (e^(-z^2) z^2 < 0.37) and __expf's, below 1e-6 together, and
+    x / 2 times it is off by half of both; against that formula in 64 bits it is within 1.5e-6 + 5e-7 z^2, relative."""
+    x = torch.cat([torch.linspace(-9, 9, 40001), torch.randn(4000) * 1e-3, torch.randn(4000) * 40, torch.randn(500) * 1e-30])
+    got, xd = _activated(x, act, config, m), x.double().numpy()
+    erfc = np.vectorize(__import__("math").erfc)
+    if act == "gelu":
+        want = 0.5 * xd * erfc(-xd / np.sqrt(2))
+    else:
+        y = -xd if act == "silu" else -2 * np.sqrt(2 / np.pi) * (xd + 0.044715 * xd ** 3)
+        with np.errstate(over="ignore"):
+            want = xd / (1 + np.exp(y))
+        normal = y < 80
+        assert (np.abs(got - want)[normal] <= ((6e-7 + 5e-7 * np.abs(y)) * np.abs(want) + 2.0 ** -126)[normal]).all()
+    assert (np.abs(got - want) <= 5e-7 * np.abs(xd) + 2.0 ** -126).all()
+    if act == "gelu":
+        z = np.abs(xd) / np.sqrt(2)
+        t = 1 / (1 + 0.3275911 * z)
+        c = t * (0.254829592 + t * (-0.284496736 + t * (1.421413741 + t * (-1.453152027 + t * 1.061405429)))) * np.exp(-z * z)
+        form = 0.5 * xd * c
+        some = (xd < 0) & (z < 8)
+        assert (np.abs(got - form)[some] <= ((1.5e-6 + 5e-7 * z * z) * np.abs(form) + 2.0 ** -126)[some]).all()
+        for low, bound in ((-3, 1e-4), (-4.5, 1e-3), (-7.5, 1e-2)):
+            assert (np.abs(got - want)[xd >= low] <= bound * np.abs(want)[xd >= low] + 2.0 ** -126).all()
+
+
+@gpu
+@pytest.mark.parametrize("config,m", [(gz.MX_CFG_SWAP_M16, 2), (gz.MX_CFG_PAIR, 130)])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_activations_of_infinities_and_large_numbers(act, config, m):
+    big = torch.tensor([float("inf"), 3e38, 1e20, -1e20, -3e38, 0.0, float("nan"), float("-inf")])
+    got = _activated(big, act, config, m)
+    assert np.array_equal(got[:3], big[:3].double().numpy())
+    if act == "none":
+        assert np.array_equal(got[3:], big[3:].double().numpy(), equal_nan=True)
+    else:
+        assert (got[3:6] == 0).all() and np.isnan(got[6])
+        # the formulas give -inf * 0 except for relu
+        assert got[7] == 0 if act == "relu" else np.isnan(got[7])
+
+
+@gpu
+@pytest.mark.parametrize("act", list(ACTS))
+def test_gated_product_of_large_gates(act):
+    """A gate far from zero: act(gate) is gate or 0, and times up exactly that."""
+    m, n, k = 17, 96, 64
+    a = gz.mx_quantize(torch.ones(m, k, device="cuda"), FP4)
+    sign = torch.where(torch.arange(n) % 2 == 0, 1.0, -1.0)[:, None].expand(n, k).contiguous().cuda()
+    g, u = gz.mx_quantize(sign, FP4), gz.mx_quantize(torch.ones(n, k, device="cuda"), FP4)
+    for config in (gz.MX_CFG_SWAP_M32, gz.MX_CFG_SINGLE):
+        d = torch.empty(m, n, device="cuda")
+        gz.MxGated(m, n, k, FP4, torch.float32, activation=ACTS[act], config=config)(a, g, u, d, 1e6, 2.0 ** -6)
+        want = np.where(np.arange(n) % 2 == 0, 64e6, -64e6 if act == "none" else 0.0)
+        assert np.array_equal(d.cpu().double().numpy(), np.broadcast_to(want, (m, n)))
