@@ -137,6 +137,9 @@ static __device__ __noinline__ bool mx_store_in_bounds(const MxParams& p, uint32
 #else
 #define GZ_MX_STORE_OK(p, row, col, ncols, rows, cols) true
 #endif
+// The same for `blocks` scales of one row from `block` on: the scale array holds whole tiles of 128 rows x 4 blocks.
+#define GZ_MX_SCALE_OK(p, row, block, blocks) \
+  GZ_MX_STORE_OK(p, row, static_cast<uint32_t>(block), blocks, ((p).m + 127u) & ~127u, static_cast<uint32_t>(4 * (p).d_groups))
 
 // The activations, within 5e-7 |x| of the exact ones.  Both GELUs are taken from the complement that is small where x is
 // negative (1 + erf and 1 + tanh would cancel there: at x = -6 nothing is left in fp32): erfc by the factors of erf_fast,
@@ -399,7 +402,7 @@ __device__ __forceinline__ void mx_store_quantized(const MxParams& p, const floa
       codes[b * (BLOCK / 8) + i] = s.byte == mx::Format<NV>::NAN_SCALE ? 0u : c;
     }
     const int64_t block = static_cast<int64_t>(col0) / BLOCK + b;
-    if (block < 4 * p.d_groups)  // rows up to the next multiple of 128 exist in the scale array
+    if (block < 4 * p.d_groups && GZ_MX_SCALE_OK(p, row, block, 1u))  // rows up to the next multiple of 128 exist in the scale array
       p.d_scales[mx::scale_word(row, block >> 2, p.d_groups) + (block & 3)] = static_cast<uint8_t>(row_ok ? s.byte : 0u);
   }
   if (row_ok && col0 < p.n && GZ_MX_STORE_OK(p, row, col0, 1u, p.m, p.n))
@@ -431,7 +434,7 @@ __device__ __forceinline__ void mx_store_quantized_row(const MxParams& p, const 
     *reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.d) + static_cast<int64_t>(row) * p.ldd + col / 2) =
         static_cast<uint16_t>(codes);
   const int64_t block = col / mx::Format<NV>::BLOCK;
-  if (live && lane % LANES == 0u && block < 4 * p.d_groups)
+  if (live && lane % LANES == 0u && block < 4 * p.d_groups && GZ_MX_SCALE_OK(p, row, block, 1u))
     p.d_scales[mx::scale_word(row, block >> 2, p.d_groups) + (block & 3)] = static_cast<uint8_t>(s.byte);
 }
 
@@ -531,7 +534,7 @@ __device__ __forceinline__ void mx_clear_scale_row(const MxParams& p, uint32_t t
   const uint32_t words = p.out_type == MX_OUT_NVFP4 ? 2u : 1u;
   for (uint32_t w = 0; w < words; ++w) {
     const int64_t g = static_cast<int64_t>(tm) * words + w;
-    if (g < p.d_groups) *reinterpret_cast<uint32_t*>(p.d_scales + mx::scale_word(row, g, p.d_groups)) = 0u;
+    if (g < p.d_groups && GZ_MX_SCALE_OK(p, row, 4 * g, 4u)) *reinterpret_cast<uint32_t*>(p.d_scales + mx::scale_word(row, g, p.d_groups)) = 0u;
   }
 }
 

@@ -239,3 +239,37 @@ def test_gated_product_of_large_gates(act):
         gz.MxGated(m, n, k, FP4, torch.float32, activation=ACTS[act], config=config)(a, g, u, d, 1e6, 2.0 ** -6)
         want = np.where(np.arange(n) % 2 == 0, 64e6, -64e6 if act == "none" else 0.0)
         assert np.array_equal(d.cpu().double().numpy(), np.broadcast_to(want, (m, n)))
+
+
+# ------------------------------------------------------------------------------------------- the checked build
+def test_every_store_of_a_scale_is_checked_in_the_debug_build():
+    """Each statement of the product kernels that writes into the scale array asks GZ_MX_SCALE_OK first."""
+    text = (api.PKG / "csrc" / "mx_gemm.cuh").read_text().splitlines()
+    stores = [i for i, line in enumerate(text) if "p.d_scales" in line]
+    assert len(stores) == 3
+    for i in stores:
+        assert "GZ_MX_SCALE_OK" in text[i - 1] + text[i], text[i]
+
+
+DEBUG_CHILD = """
+import sys
+sys.path.insert(0, {root!r})
+import gemm_zoo_b200.api as api
+api.lib_path = api.debug_lib_path  # before the first lib() call: this process runs the debug build
+import gemm_zoo_b200 as gz
+from tests import test_microscale_calls as t
+for config, m, split in [(gz.MX_CFG_SWAP_M16, 13, 4), (gz.MX_CFG_SWAP_M64, 64, 8), (gz.MX_CFG_SINGLE, 130, 4), (gz.MX_CFG_PAIR, 300, 2)]:
+    for out in t.FORMATS:
+        t.test_quantised_gated_result_with_a_shared_k_range(t.NV, out, config, m, split)
+print("DEBUG OK")
+"""
+
+
+@gpu
+def test_debug_build_refuses_no_store_of_a_scale():
+    import subprocess
+    import sys
+    from gemm_zoo_b200 import build as b
+    b.build_lib(debug=True)
+    r = subprocess.run([sys.executable, "-c", DEBUG_CHILD.format(root=str(api.PKG.parent))], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "DEBUG OK" in r.stdout, (r.stdout[-500:], r.stderr[-2000:])
