@@ -273,3 +273,31 @@ def test_debug_build_refuses_no_store_of_a_scale():
     b.build_lib(debug=True)
     r = subprocess.run([sys.executable, "-c", DEBUG_CHILD.format(root=str(api.PKG.parent))], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "DEBUG OK" in r.stdout, (r.stdout[-500:], r.stderr[-2000:])
+
+
+# ------------------------------------------------------------------------------------------- the allocator's stream
+def _owner(t):
+    """The stream whose pool a tensor's memory was taken from."""
+    at = t.data_ptr()
+    return [s["stream"] for s in torch.cuda.memory_snapshot() if s["address"] <= at < s["address"] + s["total_size"]]
+
+
+@gpu
+def test_memory_of_a_new_matrix_belongs_to_the_stream_that_writes_it():
+    """Freed memory goes back to that stream's pool, where its next use is ordered behind the call that wrote it."""
+    x = torch.randn(512, 4096, device="cuda")
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream, handle in ((side, side.cuda_stream), (side.cuda_stream, side.cuda_stream), (None, 0), (0, 0)):
+        for current in (torch.cuda.default_stream(), side, other):
+            with torch.cuda.stream(current):
+                q = gz.mx_quantize(x, NV, stream=stream)
+                assert _owner(q.codes) == [handle] and _owner(q.scales) == [handle]
+                at, size = q.codes.data_ptr(), tuple(q.codes.shape)
+                del q
+            for s in (torch.cuda.default_stream(), side, other):  # freed: handed out again on its own stream alone
+                with torch.cuda.stream(s):
+                    again = torch.empty(size, dtype=torch.uint8, device="cuda")
+                    assert (again.data_ptr() == at) <= (s.cuda_stream == handle)
+                    del again
+    torch.cuda.synchronize()
