@@ -101,22 +101,6 @@ __device__ __forceinline__ uint32_t pack8(float v0, float v1, float v2, float v3
   return r;
 }
 
-// One value in code units -> its e2m1 code in the low nibble.
-__device__ __forceinline__ uint32_t pack1(float v) {
-  uint32_t r;
-  asm("{\n\t"
-      ".reg .b8 b0, z;\n\t"
-      ".reg .b32 t;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "mov.b32 t, 0;\n\t"
-      "mov.b32 {z, _, _, _}, t;\n\t"
-      "mov.b32 %0, {b0, z, z, z};\n\t"
-      "}"
-      : "=r"(r)
-      : "f"(v), "f"(0.0f));
-  return r;
-}
-
 // Eight e2m1 codes -> eight fp32 values (exact).
 __device__ __forceinline__ void unpack8(uint32_t codes, float (&v)[8]) {
   uint32_t h[4];

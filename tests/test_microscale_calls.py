@@ -301,3 +301,15 @@ def test_memory_of_a_new_matrix_belongs_to_the_stream_that_writes_it():
                     assert (again.data_ptr() == at) <= (s.cuda_stream == handle)
                     del again
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------- nothing unreached
+def test_every_function_of_the_microscaled_sources_is_called():
+    import re
+    files = [f for f in (api.PKG / "csrc").rglob("*") if f.suffix in (".cuh", ".cu", ".h")]
+    text = "\n".join(f.read_text() for f in files)
+    for f in files:
+        if not f.name.startswith("mx_"):
+            continue
+        for name in re.findall(r"__device__ (?:__forceinline__|__noinline__)?\s*[\w:<>]+\s+(\w+)\(", f.read_text()):
+            assert len(re.findall(rf"\b{name}\b", re.sub(r"//.*", "", text))) > 1, name
