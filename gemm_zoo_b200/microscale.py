@@ -146,6 +146,10 @@ class MxMatrix:
 def tile_scales(linear, format):
     """rows x blocks scale bytes (one row after the other, as checkpoints hold them) -> the tiled array."""
     import torch
+    if format not in (MX_FP4, MX_NVFP4):
+        raise ValueError("tile_scales: format must be one of MX_FP4, MX_NVFP4")
+    if linear.dim() != 2 or linear.element_size() != 1 or linear.numel() == 0:
+        raise ValueError("tile_scales: rows x blocks scale bytes are needed")
     rows, blocks = linear.shape
     rg, bg = -(-rows // 128), -(-blocks // 4)
     s = torch.zeros(rg * 128, bg * 4, dtype=torch.uint8, device=linear.device)

@@ -313,3 +313,17 @@ def test_every_function_of_the_microscaled_sources_is_called():
             continue
         for name in re.findall(r"__device__ (?:__forceinline__|__noinline__)?\s*[\w:<>]+\s+(\w+)\(", f.read_text()):
             assert len(re.findall(rf"\b{name}\b", re.sub(r"//.*", "", text))) > 1, name
+
+
+# ------------------------------------------------------------------------------------------- scales from elsewhere
+def test_tile_scales_checks_its_arguments():
+    ok = torch.zeros(3, 5, dtype=torch.uint8)
+    for fmt in FORMATS:
+        assert gz.tile_scales(ok, fmt).numel() == 1024
+        assert gz.tile_scales(ok.view(torch.float8_e4m3fn), fmt).numel() == 1024
+        for bad in (ok[0], ok[:, :, None], ok.half(), ok[:0], ok[:, :0]):
+            with pytest.raises(ValueError):
+                gz.tile_scales(bad, fmt)
+    for fmt in (0, 3, 15, 18, None):
+        with pytest.raises(ValueError):
+            gz.tile_scales(ok, fmt)
