@@ -83,8 +83,9 @@ typedef struct gz_mx_desc {
   int32_t gated;        /* 0: gz_mx_gemm_run, 1: gz_mx_gated_run */
   int32_t device;
   int32_t config;       /* gz_mx_config */
-  int32_t split;        /* CTAs (pair tiles: pairs) that share a tile's K range: 1, 2, 4 or 8
-                           (at most one per 32 output columns of the tile, and eight CTAs); 0 = chosen */
+  int32_t split;        /* CTAs (pair tiles: pairs) that share a tile's K range: 1, 2, 4 or 8, at most one
+                           per 256 of K and eight CTAs, in row tiles (PAIR, SINGLE and their N128) also at
+                           most one per 32 output columns of the tile; 0 = chosen */
   uint32_t flags;       /* 0 or GZ_FLAG_TEST_WITHHOLD_ACC_READY */
   int64_t m, n, k;
   int64_t pitch_a, pitch_b; /* bytes between rows of codes (gated: pitch_b for gate and up); 0 = packed */

@@ -327,3 +327,16 @@ def test_tile_scales_checks_its_arguments():
     for fmt in (0, 3, 15, 18, None):
         with pytest.raises(ValueError):
             gz.tile_scales(ok, fmt)
+
+
+# ------------------------------------------------------------------------------------------- limits of the split
+@pytest.mark.parametrize("config,gated,most", [
+    (gz.MX_CFG_PAIR, False, 4), (gz.MX_CFG_PAIR, True, 4), (gz.MX_CFG_SINGLE, False, 8), (gz.MX_CFG_SINGLE, True, 4),
+    (gz.MX_CFG_PAIR_N128, False, 4), (gz.MX_CFG_SINGLE_N128, False, 4), (gz.MX_CFG_SWAP_M16, False, 8), (gz.MX_CFG_SWAP_M16, True, 8),
+    (gz.MX_CFG_SWAP_M32, False, 8), (gz.MX_CFG_SWAP_M64, True, 8)])
+def test_limits_of_the_split_are_those_of_the_header(config, gated, most):
+    """A tile's output columns over 32 (row tiles), eight CTAs, and one part of K at least per CTA."""
+    for split in (1, 2, 4, 8):
+        for blocks in (1, 2, 3, 7, 8):
+            d = gz.MxDesc.make(FP4, gz.DT_BF16, 16, 512, 256 * blocks, gated, config=config, split=split)
+            assert (gz.mx_validate(d)[0] == api.GZ_OK) == (split <= most and split <= blocks)
