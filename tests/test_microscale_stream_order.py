@@ -98,3 +98,26 @@ def test_bias_of_a_16_bit_product_written_by_the_product_before(config, m):
         second.run_ex(a, w, None, out, 1.0, 0.0, bias=v.view(-1))
     torch.cuda.synchronize()
     assert all(torch.equal(out, want[i % 4]) for i, out in enumerate(d))
+
+
+@pytest.mark.parametrize("config,m,split", [(gz.MX_CFG_AUTO, 1, 0), (gz.MX_CFG_SWAP_M64, 40, 8), (gz.MX_CFG_SINGLE, 130, 4), (gz.MX_CFG_PAIR, 300, 2),
+                                            (gz.MX_CFG_PAIR, 2500, 1)])
+def test_repeated_calls_give_the_same_bits(config, m, split):
+    """Sums are taken in one order whatever runs when: a feed-forward layer of arbitrary values, again and again."""
+    n, k = 640, 2048
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    g, u, w = (gz.mx_quantize(torch.randn(s, device="cuda") * 5, NV) for s in ((n, k), (n, k), (k, n)))
+    q, h = gz.MxMatrix.empty(m, k, NV), gz.MxMatrix.empty(m, n, NV)
+    gated, down = gz.MxGated(m, n, k, NV, NV, config=config, split=split), gz.MxGemm(m, k, n, NV, torch.float32)
+    y = [torch.empty(m, k, device="cuda") for _ in range(12)]
+    codes, scales = [], []
+    for out in y:
+        gz.mx_quantize(x, NV, out=q)
+        gated(q, g, u, h, 0.02, 0.02)
+        down(h, w, None, out, 0.02, 0.0)
+        codes.append(h.codes.clone())
+        scales.append(h.scales.clone())
+    torch.cuda.synchronize()
+    assert float(y[0].abs().max()) > 0
+    for got in (y, codes, scales):
+        assert all(torch.equal(v, got[0]) for v in got)
