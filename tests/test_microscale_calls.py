@@ -340,3 +340,18 @@ def test_limits_of_the_split_are_those_of_the_header(config, gated, most):
         for blocks in (1, 2, 3, 7, 8):
             d = gz.MxDesc.make(FP4, gz.DT_BF16, 16, 512, 256 * blocks, gated, config=config, split=split)
             assert (gz.mx_validate(d)[0] == api.GZ_OK) == (split <= most and split <= blocks)
+
+
+# ------------------------------------------------------------------------------------------- lengths of one
+@gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("config", [gz.MX_CFG_AUTO, gz.MX_CFG_SWAP_M16, gz.MX_CFG_SWAP_M64, gz.MX_CFG_SINGLE, gz.MX_CFG_SINGLE_N128, gz.MX_CFG_PAIR,
+                                    gz.MX_CFG_PAIR_N128])
+def test_products_of_single_elements(fmt, config):
+    for m, n, k in [(1, 1, 1), (1, 1, 2), (3, 1, 3), (1, 5, 1), (2, 2, 15), (1, 1, 257), (1, 129, 1)]:
+        (a, av), (b, bv) = _mx(m, k, fmt, 1, True), _mx(n, k, fmt, 2, True)
+        for dtype in (torch.float32, torch.float16):
+            full, d = _out(m, n, n + 3, dtype)
+            gz.MxGemm(m, n, k, fmt, dtype, ldd=n + 3, config=config)(a, b, None, d[:, :n], 1.0, 0.0)
+            torch.cuda.synchronize()
+            assert np.array_equal(d[:, :n].cpu().double().numpy(), av @ bv.T) and _guards_intact(full, m, n)
