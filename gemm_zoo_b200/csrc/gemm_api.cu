@@ -987,8 +987,13 @@ gz_status run_impl(gz_plan* pl, const void* a, const void* b, const void* c, voi
   p.beta_i = bi;
   p.c = beta_zero ? nullptr : c;
   p.d = d;
-  p.c_vec_ok = (c && reinterpret_cast<uintptr_t>(c) % 16 == 0 && (pr.d.ldc * pr.out_size) % 16 == 0) ? 1u : 0u;
-  p.d_vec_ok = (reinterpret_cast<uintptr_t>(d) % 16 == 0 && (pr.d.ldd * pr.out_size) % 16 == 0) ? 1u : 0u;
+  // 16-byte accesses: every row of every problem of the batch starts at a multiple of 16 bytes
+  auto rows_aligned = [&](const void* base, int64_t ld, int64_t stride) {
+    return base && reinterpret_cast<uintptr_t>(base) % 16 == 0 && (ld * pr.out_size) % 16 == 0 &&
+           (pr.d.batch == 1 || (stride * pr.out_size) % 16 == 0);
+  };
+  p.c_vec_ok = rows_aligned(c, pr.d.ldc, pr.d.stride_c) ? 1u : 0u;
+  p.d_vec_ok = rows_aligned(d, pr.d.ldd, pr.d.stride_d) ? 1u : 0u;
   if (p.epilogue_tma && reinterpret_cast<uintptr_t>(d) % 16 != 0) p.epilogue_tma = 0;
   if (epi_flags) {
     p.epi_flags = epi_flags;
